@@ -50,6 +50,14 @@ extern "C" {
 #define RLT_E_DEVICE -7
 #define RLT_E_SCRATCH -8
 
+/* activations of the projection operators */
+#define RLT_ACT_NONE 0
+#define RLT_ACT_SILU 1      /* x / (1 + exp(-x)) */
+#define RLT_ACT_GELU 2      /* x (1 + erf(x / sqrt 2)) / 2 */
+#define RLT_ACT_GELU_TANH 3 /* x (1 + tanh(sqrt(2 / pi) (x + 0.044715 x^3))) / 2 */
+#define RLT_ACT_RELU 4      /* max(x, 0) */
+#define RLT_ACT_SIGMOID 5   /* 1 / (1 + exp(-x)) */
+
 /* status bits */
 #define RLT_STATUS_BAD_LENGTH 1
 #define RLT_STATUS_BAD_BLOCK 2
@@ -58,6 +66,7 @@ extern "C" {
 #define RLT_STATUS_BAD_SEQUENCE 16
 #define RLT_STATUS_TIMEOUT 32 /* a bounded wait inside a tensor-core kernel gave up */
 #define RLT_STATUS_LAYOUT 64  /* a tensor-core kernel found its shared memory misaligned */
+#define RLT_STATUS_BAD_TOKEN 128 /* a token to score lies outside the vocabulary */
 
 /* Library version (major*10000 + minor*100 + patch). */
 int rlt_version(void);
@@ -391,6 +400,72 @@ int rlt_rope_write_kv(const void* qkv, const int64_t* positions, const float* in
  * to the dtype). Replaces: vllm_rlt/models/ouro.py:122-123. */
 int rlt_silu_mul(const void* gate_up, void* out, int32_t dtype, int32_t rows,
                  int32_t intermediate, int64_t in_stride, int64_t out_stride, void* stream);
+
+/* ---- projections ---- */
+
+/* Scratch of rlt_linear and rlt_gated_linear, in bytes: copies of x and of the
+ * weights in rows of whole 16-byte units, for 16-bit operands that are not laid
+ * out so (a pointer that is not 16-byte aligned, a stride that is not a
+ * multiple of 8 elements or shorter than its row). 0 when none is needed, and
+ * always for fp32. `gated`: 0 or 1; out_features counts one half then. */
+size_t rlt_linear_workspace_bytes(const void* x, const void* weight, int32_t dtype, int32_t rows,
+                                  int32_t in_features, int32_t out_features, int32_t gated,
+                                  int64_t x_row_stride, int64_t weight_out_stride,
+                                  int64_t weight_in_stride);
+
+/* Matrix product with its epilogue, in one launch:
+ *   out[r, n] = act(sum_k x[r, k] weight[n, k] + bias[n]) + residual[r, n]
+ * accumulated in fp32 and rounded once to the dtype. weight is [out, in] with
+ * either dimension contiguous (weight_in_stride 1, or weight_out_stride 1: the
+ * transposed view of an [in, out] tensor); the last dimension of x, residual
+ * and out is contiguous. bias and residual may be NULL; out may be the same
+ * tensor as residual and overlaps nothing else. in_features >= 1; rows or
+ * out_features of 0 launch nothing. act: RLT_ACT_*. A row's result depends on
+ * that row, the weights, and the launch shape only, and repeats bit for bit.
+ * bf16 and fp16 run on the tensor cores, fp32 in fp32 multiply-adds.
+ * Replaces the projections of vllm_rlt/models/ouro.py:96-123 with what follows
+ * them, and the exit gate's product, bias and sigmoid (:209-217). */
+int rlt_linear(const void* x, const void* weight, const void* bias, const void* residual,
+               void* out, void* workspace, size_t workspace_bytes, int32_t* status, int32_t dtype,
+               int32_t rows, int32_t in_features, int32_t out_features, int32_t activation,
+               int64_t x_row_stride, int64_t weight_out_stride, int64_t weight_in_stride,
+               int64_t residual_row_stride, int64_t out_row_stride, void* stream);
+
+/* Gated product: weight is [2 * out_features, in], gate rows then up rows,
+ *   out[r, n] = act(x[r] . weight[n]) * (x[r] . weight[out_features + n])
+ * with both products, the activation and the multiplication in fp32 and one
+ * rounding to the dtype. Otherwise as rlt_linear.
+ * Replaces: vllm_rlt/models/ouro.py:115-123 up to the down projection (where
+ * each of the three steps rounds to the dtype). */
+int rlt_gated_linear(const void* x, const void* weight, void* out, void* workspace,
+                     size_t workspace_bytes, int32_t* status, int32_t dtype, int32_t rows,
+                     int32_t in_features, int32_t out_features, int32_t activation,
+                     int64_t x_row_stride, int64_t weight_out_stride, int64_t weight_in_stride,
+                     int64_t out_row_stride, void* stream);
+
+/* Scratch of rlt_vocab_head, in bytes: per (row, vocabulary tile) records,
+ * and aligned copies as for rlt_linear. */
+size_t rlt_vocab_head_workspace_bytes(const void* hidden, const void* weight, int32_t dtype,
+                                      int32_t rows, int32_t in_features, int32_t vocab,
+                                      int64_t hidden_row_stride, int64_t weight_out_stride,
+                                      int64_t weight_in_stride);
+
+/* Language-model head without its logits l[r, v] = hidden[r] . weight[v]
+ * (fp32, never stored): each vocabulary tile leaves its largest logit, sum of
+ * exponentials and scored logit per row, and a second launch joins them.
+ *   tokens NULL: out_tokens[r] = the lowest v that attains max_v l[r, v] (as
+ *     torch.argmax: a NaN counts as largest), logprobs[r] = log softmax there;
+ *   else: logprobs[r] = log softmax(l[r])[tokens[r]] and out_tokens is unused;
+ *     0 where tokens[r] is negative (a row with nothing to score); NaN and
+ *     status bit RLT_STATUS_BAD_TOKEN where tokens[r] >= vocab.
+ * logprobs fp32, token ids int64. vocab >= 1.
+ * Replaces: the LM head and argmax of vllm_rlt/worker/model_runner.py:420-427 and :602-618;
+ * the reference has no counterpart of the scored form. */
+int rlt_vocab_head(const void* hidden, const void* weight, const int64_t* tokens,
+                   int64_t* out_tokens, float* logprobs, void* workspace, size_t workspace_bytes,
+                   int32_t* status, int32_t dtype, int32_t rows, int32_t in_features,
+                   int32_t vocab, int64_t hidden_row_stride, int64_t weight_out_stride,
+                   int64_t weight_in_stride, void* stream);
 
 /* KV page transport for prefill/decode disaggregation: copy byte segments
  * segments[i*3 + 0..2] = {source address, destination address, bytes}

@@ -11,6 +11,10 @@ Public surface (mirrors vllm_rlt/kernels):
   * ``write_kv`` / ``finalize`` -- KV page write and LAST-EXITED exit copy;
   * ``metadata``, ``gather``, ``scatter``, ``stage_prefill``,
     ``expand_prefill`` -- routing and prefill-metadata kernels;
+  * ``linear`` / ``gated_linear`` -- projections with bias, activation and
+    residual, or with the gate's activation and product, in the same kernel;
+  * ``greedy_tokens`` / ``token_logprobs`` -- language-model head reduced to
+    the next token, or to given tokens' log-probabilities, without its logits;
   * ``install`` -- put the backend into a reference KV cache manager.
 
 Importing the package does not initialise CUDA; the shared library is loaded
@@ -33,4 +37,10 @@ from .kernels.shared_prefix import (  # noqa: F401
     plan_shared_prefix,
 )
 from .kernels.prefill_metadata import expand_prefill, stage_prefill  # noqa: F401
+from .kernels.projections import (  # noqa: F401
+    gated_linear,
+    greedy_tokens,
+    linear,
+    token_logprobs,
+)
 from .kernels.routing import gather, metadata, scatter  # noqa: F401

@@ -39,6 +39,7 @@ STATUS_BITS = {
     16: "packed-prefill metadata inconsistent",
     32: "a bounded wait in a kernel timed out (the call's output is void)",
     64: "a tensor-core kernel found its shared memory misaligned",
+    128: "a token to score lies outside the vocabulary",
 }
 
 _i32, _i64, _f32, _sz, _p = (
@@ -96,6 +97,11 @@ SIGNATURES = {
     "rlt_rms_norm2": (_i32, [_p] * 6 + [_i32] * 3 + [_f32] + [_i64] * 4 + [_p]),
     "rlt_rope_write_kv": (_i32, [_p] * 9 + [_i32] * 7 + [_i64] * 8 + [_p]),
     "rlt_silu_mul": (_i32, [_p, _p, _i32, _i32, _i32, _i64, _i64, _p]),
+    "rlt_linear_workspace_bytes": (_sz, [_p, _p] + [_i32] * 5 + [_i64] * 3),
+    "rlt_linear": (_i32, [_p] * 6 + [_sz, _p] + [_i32] * 5 + [_i64] * 5 + [_p]),
+    "rlt_gated_linear": (_i32, [_p] * 4 + [_sz, _p] + [_i32] * 5 + [_i64] * 4 + [_p]),
+    "rlt_vocab_head_workspace_bytes": (_sz, [_p, _p] + [_i32] * 4 + [_i64] * 3),
+    "rlt_vocab_head": (_i32, [_p] * 6 + [_sz, _p] + [_i32] * 4 + [_i64] * 3 + [_p]),
     "rlt_copy_segments": (_i32, [_p, _i32, _i64, _p, _p]),
     "rlt_enable_peer_access": (_i32, [_i32]),
     "rlt_gather": (_i32, [_p, _p, _p, _i32, _i32, _i32, _i32, _i64, _i64, _p]),

@@ -25,6 +25,7 @@ constexpr int32_t kStatusBadOffset = 4;   // in-page offset outside [0, page)
 constexpr int32_t kStatusBadSlot = 8;     // descriptor slot / depth outside the resident tables
 constexpr int32_t kStatusBadSequence = 16;  // packed-prefill sequence metadata inconsistent
 constexpr int32_t kStatusTimeout = 32;      // a bounded wait gave up (the call's output is void)
+constexpr int32_t kStatusBadToken = 128;    // a token to score outside the vocabulary
 
 // Inter-CTA hand-off through global memory (gpu scope).
 __device__ __forceinline__ int ld_acquire_gpu(const int* ptr) {
