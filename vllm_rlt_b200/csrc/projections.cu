@@ -326,18 +326,102 @@ int run_fma(const Problem& p, cudaStream_t stream) {
   }
 }
 
-template <Kind kKind>
-int dispatch(const Problem& p, int32_t dtype, cudaStream_t stream) {
-  switch (dtype) {
-    case RLT_F32: return run_fma<float, kKind>(p, stream);
-    case RLT_F16: return run_fma<__half, kKind>(p, stream);
-    default: return run_fma<__nv_bfloat16, kKind>(p, stream);
+// ---- 16-bit operands for the tensor cores -------------------------------------
+
+int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// What TMA asks of an operand of `lines` lines of `line` elements: a 16-byte
+// aligned start and a stride of whole 16-byte units. A stride shorter than a
+// line (a broadcast operand) is copied too.
+bool tma_ready(const void* base, int line, int lines, int64_t stride) {
+  return aligned16(base) && (lines == 1 || (stride % 8 == 0 && stride >= line));
+}
+
+struct Layout {  // of the weights: lines along the contiguous dimension
+  int line, lines;
+  int64_t stride;
+};
+Layout weight_layout(const Problem& p) {
+  return p.w_ks == 1 ? Layout{p.inner, p.outer, p.w_ns} : Layout{p.outer, p.inner, p.w_ks};
+}
+
+bool x_ready(const Problem& p) { return tma_ready(p.x, p.inner, p.rows, p.x_rs); }
+bool w_ready(const Problem& p) {
+  const Layout l = weight_layout(p);
+  return tma_ready(p.w, l.line, l.lines, l.stride) &&
+         (p.w_up == nullptr || tma_ready(p.w_up, l.line, l.lines, l.stride));
+}
+
+size_t copies_bytes(const Problem& p, int32_t dtype) {
+  if (dtype == RLT_F32) return 0;
+  const Layout l = weight_layout(p);
+  size_t bytes = 0;
+  if (!x_ready(p)) bytes += static_cast<size_t>(round8(p.inner)) * p.rows * 2;
+  if (!w_ready(p)) bytes += static_cast<size_t>(round8(l.line)) * l.lines * (p.w_up ? 4 : 2);
+  return bytes;
+}
+
+// dst[line][0 .. pitch) = src[line * stride ..][0 .. length), 16-bit elements;
+// what lies past `length` is never read.
+__global__ void __launch_bounds__(256) align_kernel(const uint16_t* __restrict__ src,
+                                                    uint16_t* __restrict__ dst, int length,
+                                                    int lines, int64_t stride, int pitch) {
+  const int units = pitch / 8;
+  const int64_t total = static_cast<int64_t>(units) * lines;
+  for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
+    const int64_t line = i / units;
+    const int c = static_cast<int>(i - line * units) * 8;
+    const uint16_t* s = src + line * stride + c;
+    uint32_t v[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (c + e < length) v[e / 2] |= static_cast<uint32_t>(s[e]) << (e % 2 * 16);
+    st_vec(dst + line * pitch + c, make_uint4(v[0], v[1], v[2], v[3]));
   }
 }
 
-int vocab_tile(int32_t dtype, int rows, int vocab) {
-  (void)dtype;
-  return fma_tile(rows, vocab) == 2 ? 128 : 64;
+int align_copy(const void*& base, int64_t& stride, int length, int lines, char*& at,
+               cudaStream_t stream) {
+  const int64_t pitch = round8(length);
+  if (pitch > INT32_MAX) return RLT_E_SHAPE;
+  const int64_t blocks = (pitch / 8 * lines + 255) / 256;
+  align_kernel<<<static_cast<unsigned>(blocks < 16 * sm_count() ? blocks : 16 * sm_count()), 256, 0,
+                 stream>>>(static_cast<const uint16_t*>(base), reinterpret_cast<uint16_t*>(at),
+                           length, lines, stride, static_cast<int>(pitch));
+  base = at;
+  stride = pitch;
+  at += pitch * lines * 2;
+  return launch_status(cudaGetLastError());
+}
+
+template <Kind kKind>
+int dispatch(Problem p, int32_t dtype, char* copies, cudaStream_t stream) {
+  if (dtype == RLT_F32) return run_fma<float, kKind>(p, stream);
+  if (!x_ready(p))
+    if (const int rc = align_copy(p.x, p.x_rs, p.inner, p.rows, copies, stream)) return rc;
+  if (!w_ready(p)) {
+    const Layout l = weight_layout(p);
+    int64_t stride = l.stride;
+    if (p.w_up != nullptr) {
+      stride = l.stride;
+      if (const int rc = align_copy(p.w_up, stride, l.line, l.lines, copies, stream)) return rc;
+      stride = l.stride;
+    }
+    if (const int rc = align_copy(p.w, stride, l.line, l.lines, copies, stream)) return rc;
+    (p.w_ks == 1 ? p.w_ns : p.w_ks) = stride;
+  }
+  // one line: its stride is never used, but has to be one that TMA accepts
+  if (p.rows == 1) p.x_rs = round8(p.inner);
+  if (p.w_ks == 1 && p.outer == 1) p.w_ns = round8(p.inner);
+  if (p.w_ks != 1 && p.inner == 1) p.w_ks = round8(p.outer);
+  return run_tc(kKind, p, dtype, sm_count(), stream);
+}
+
+// Columns per vocabulary tile of the kernel that the call will run.
+int vocab_tile(const Problem& p, int32_t dtype) {
+  if (dtype != RLT_F32) return tc_vocab_tile(p, sm_count());
+  return fma_tile(p.rows, p.outer) == 2 ? 128 : 64;
 }
 
 bool known(int32_t dtype) { return dtype == RLT_F32 || dtype == RLT_F16 || dtype == RLT_BF16; }
@@ -349,6 +433,28 @@ int check(int32_t dtype, int32_t rows, int32_t inner, int32_t outer, int32_t act
     return RLT_E_SHAPE;
   if (w_ns != 1 && w_ks != 1) return RLT_E_SHAPE;
   return RLT_OK;
+}
+
+Problem problem(const void* x, const void* w, int32_t rows, int32_t inner, int32_t outer,
+                int64_t x_rs, int64_t w_ns, int64_t w_ks) {
+  Problem p{};
+  p.x = x;
+  p.w = w;
+  p.rows = rows;
+  p.inner = inner;
+  p.outer = outer;
+  p.x_rs = x_rs;
+  p.w_ns = w_ns;
+  p.w_ks = w_ks;
+  return p;
+}
+
+const void* up_rows(const void* weight, int32_t dtype, int32_t out_features, int64_t w_ns) {
+  return static_cast<const char*>(weight) + w_ns * out_features * (dtype == RLT_F32 ? 4 : 2);
+}
+
+size_t parts_bytes(const Problem& p, int32_t dtype) {
+  return static_cast<size_t>(p.rows) * ceil_div(p.outer, vocab_tile(p, dtype)) * sizeof(VocabPart);
 }
 
 }  // namespace
@@ -363,7 +469,14 @@ extern "C" size_t rlt_linear_workspace_bytes(const void* x, const void* weight, 
                                              int32_t out_features, int32_t gated,
                                              int64_t x_row_stride, int64_t weight_out_stride,
                                              int64_t weight_in_stride) {
-  return 0;
+  if (check(dtype, rows, in_features, out_features, RLT_ACT_NONE, weight_out_stride,
+            weight_in_stride) ||
+      rows == 0 || out_features == 0)
+    return 0;
+  Problem p = problem(x, weight, rows, in_features, out_features, x_row_stride, weight_out_stride,
+                      weight_in_stride);
+  if (gated) p.w_up = up_rows(weight, dtype, out_features, weight_out_stride);
+  return copies_bytes(p, dtype);
 }
 
 extern "C" int rlt_linear(const void* x, const void* weight, const void* bias,
@@ -377,12 +490,20 @@ extern "C" int rlt_linear(const void* x, const void* weight, const void* bias,
                            weight_in_stride))
     return rc;
   if (rows == 0 || out_features == 0) return RLT_OK;
-  Problem p{x,           weight,       nullptr,      bias,
-            residual,    out,          status,       rows,
-            in_features, out_features, activation,   x_row_stride,
-            weight_out_stride, weight_in_stride, residual_row_stride, out_row_stride,
-            nullptr,     nullptr,      0};
-  return dispatch<kLinear>(p, dtype, static_cast<cudaStream_t>(stream));
+  Problem p = problem(x, weight, rows, in_features, out_features, x_row_stride, weight_out_stride,
+                      weight_in_stride);
+  p.bias = bias;
+  p.residual = residual;
+  p.out = out;
+  p.status = status;
+  p.act = activation;
+  p.r_rs = residual_row_stride;
+  p.o_rs = out_row_stride;
+  const size_t need = copies_bytes(p, dtype);
+  if (need > 0 && (!aligned16(workspace) || workspace == nullptr || workspace_bytes < need))
+    return RLT_E_WORKSPACE;
+  return dispatch<kLinear>(p, dtype, static_cast<char*>(workspace),
+                           static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int rlt_gated_linear(const void* x, const void* weight, void* out, void* workspace,
@@ -395,14 +516,18 @@ extern "C" int rlt_gated_linear(const void* x, const void* weight, void* out, vo
                            weight_in_stride))
     return rc;
   if (rows == 0 || out_features == 0) return RLT_OK;
-  const int es = dtype == RLT_F32 ? 4 : 2;
-  const void* up = static_cast<const char*>(weight) + weight_out_stride * out_features * es;
-  Problem p{x,           weight,       up,           nullptr,
-            nullptr,     out,          status,       rows,
-            in_features, out_features, activation,   x_row_stride,
-            weight_out_stride, weight_in_stride, 0, out_row_stride,
-            nullptr,     nullptr,      0};
-  return dispatch<kGated>(p, dtype, static_cast<cudaStream_t>(stream));
+  Problem p = problem(x, weight, rows, in_features, out_features, x_row_stride, weight_out_stride,
+                      weight_in_stride);
+  p.w_up = up_rows(weight, dtype, out_features, weight_out_stride);
+  p.out = out;
+  p.status = status;
+  p.act = activation;
+  p.o_rs = out_row_stride;
+  const size_t need = copies_bytes(p, dtype);
+  if (need > 0 && (!aligned16(workspace) || workspace == nullptr || workspace_bytes < need))
+    return RLT_E_WORKSPACE;
+  return dispatch<kGated>(p, dtype, static_cast<char*>(workspace),
+                          static_cast<cudaStream_t>(stream));
 }
 
 extern "C" size_t rlt_vocab_head_workspace_bytes(const void* hidden, const void* weight,
@@ -410,9 +535,12 @@ extern "C" size_t rlt_vocab_head_workspace_bytes(const void* hidden, const void*
                                                  int32_t vocab, int64_t hidden_row_stride,
                                                  int64_t weight_out_stride,
                                                  int64_t weight_in_stride) {
-  if (!known(dtype) || rows <= 0 || vocab <= 0) return 0;
-  return static_cast<size_t>(rows) * ceil_div(vocab, vocab_tile(dtype, rows, vocab)) *
-         sizeof(VocabPart);
+  if (check(dtype, rows, in_features, vocab, RLT_ACT_NONE, weight_out_stride, weight_in_stride) ||
+      rows == 0 || vocab == 0)
+    return 0;
+  const Problem p = problem(hidden, weight, rows, in_features, vocab, hidden_row_stride,
+                            weight_out_stride, weight_in_stride);
+  return parts_bytes(p, dtype) + copies_bytes(p, dtype);
 }
 
 extern "C" int rlt_vocab_head(const void* hidden, const void* weight, const int64_t* tokens,
@@ -425,19 +553,20 @@ extern "C" int rlt_vocab_head(const void* hidden, const void* weight, const int6
     return rc;
   if (vocab == 0) return RLT_E_SHAPE;
   if (rows == 0) return RLT_OK;
-  const size_t need = rlt_vocab_head_workspace_bytes(hidden, weight, dtype, rows, in_features,
-                                                     vocab, hidden_row_stride, weight_out_stride,
-                                                     weight_in_stride);
-  if (workspace == nullptr || workspace_bytes < need) return RLT_E_WORKSPACE;
+  Problem p = problem(hidden, weight, rows, in_features, vocab, hidden_row_stride,
+                      weight_out_stride, weight_in_stride);
+  const size_t parts = parts_bytes(p, dtype);
+  if (workspace == nullptr || !aligned16(workspace) ||
+      workspace_bytes < parts + copies_bytes(p, dtype))
+    return RLT_E_WORKSPACE;
+  p.status = status;
+  p.tokens = tokens;
+  p.parts = static_cast<VocabPart*>(workspace);
+  p.tiles = ceil_div(vocab, vocab_tile(p, dtype));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int tiles = ceil_div(vocab, vocab_tile(dtype, rows, vocab));
-  Problem p{hidden,      weight,       nullptr,      nullptr,
-            nullptr,     nullptr,      status,       rows,
-            in_features, vocab,        RLT_ACT_NONE, hidden_row_stride,
-            weight_out_stride, weight_in_stride, 0, 0,
-            tokens,      static_cast<VocabPart*>(workspace), tiles};
-  if (const int rc = dispatch<kVocab>(p, dtype, s)) return rc;
+  if (const int rc = dispatch<kVocab>(p, dtype, static_cast<char*>(workspace) + parts, s))
+    return rc;
   vocab_join_kernel<<<ceil_div(rows, 8), 256, 0, s>>>(p.parts, tokens, out_tokens, logprobs,
-                                                      status, rows, tiles, vocab);
+                                                      status, rows, p.tiles, vocab);
   return launch_status(cudaGetLastError());
 }
