@@ -13,6 +13,12 @@
 // contiguous a stage holds them K-major (128-byte rows of 64 input features),
 // else MN-major (blocks of 64 output features by 64 input features). Rows and
 // features outside the operands arrive as zeros.
+//
+// stream_kernel: few activation rows. The weights are what has to be read, so
+// here they are the 128-row operand and the activations the narrow one (16 to
+// 64 columns): a CTA streams 128 output features over its share of the input
+// features, a cluster of up to 8 CTAs shares a feature tile, and their partial
+// sums meet in distributed shared memory.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -322,6 +328,198 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
   }
 }
 
+// ---- few rows -----------------------------------------------------------------
+
+constexpr int kStreamRows = 64;     // activation rows that stream_kernel takes
+constexpr int kStreamStages = 12;
+constexpr int kStreamFeatures = 128;
+
+struct StreamParams {
+  CUtensorMap map_x, map_w, map_up;
+  Problem p;
+  int stages;
+  int stage_bytes;
+  int cols;    // activation rows rounded up to the instruction's 16
+  int w_mn;
+  int splits;  // CTAs per feature tile
+};
+
+template <typename T, Kind kKind>
+__global__ void __launch_bounds__(kThreads) stream_kernel(const __grid_constant__ StreamParams g) {
+  constexpr int kOps = kKind == kGated ? 2 : 1;
+  constexpr int kBytesW = kStreamFeatures * kBlockK * 2;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full[kStreamStages], empty[kStreamStages], acc_full;
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int aborted;
+  const Problem& p = g.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const int rank = g.splits > 1 ? static_cast<int>(tc::cluster_rank()) : 0;
+  const int n0 = blockIdx.x / g.splits * kStreamFeatures;
+  const int kblocks = (p.inner + kBlockK - 1) / kBlockK;
+  const int kb0 = static_cast<int>(static_cast<int64_t>(kblocks) * rank / g.splits);
+  const int kb1 = static_cast<int>(static_cast<int64_t>(kblocks) * (rank + 1) / g.splits);
+  constexpr uint32_t kTmemCols = kOps * kStreamRows;  // 64 or 128, powers of two
+
+  if (threadIdx.x == 128) {
+    tc::prefetch_tensormap(&g.map_w);
+    tc::prefetch_tensormap(&g.map_x);
+    if (kOps == 2) tc::prefetch_tensormap(&g.map_up);
+    for (int i = 0; i < g.stages; ++i) {
+      tc::mbar_init(&full[i], 1);
+      tc::mbar_init(&empty[i], 1);
+    }
+    tc::mbar_init(&acc_full, 1);
+    aborted = 0;
+    tc::fence_mbar_init();
+  }
+  if (warp == 5) tc::tmem_alloc(&tmem_slot, kTmemCols);
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  bool ok = true;
+
+  if (warp == 4) {
+    if (lane == 0) {
+      const uint32_t bytes = kOps * kBytesW + g.cols * 128;
+      for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {
+        const int s = it % g.stages;
+        if (it >= g.stages && !tc::mbar_wait(&empty[s], (it / g.stages - 1) & 1, kWaitLimit)) {
+          ok = false;
+          break;
+        }
+        uint8_t* w = smem + s * g.stage_bytes;
+        tc::mbar_expect_tx(&full[s], bytes);
+        for (int op = 0; op < kOps; ++op) {
+          const CUtensorMap* map = op ? &g.map_up : &g.map_w;
+          uint8_t* dst = w + op * kBytesW;
+          if (g.w_mn) {
+            tc::tma_load_2d(dst, map, &full[s], n0, kb * kBlockK);
+            tc::tma_load_2d(dst + 8192, map, &full[s], n0 + 64, kb * kBlockK);
+          } else {
+            tc::tma_load_2d(dst, map, &full[s], kb * kBlockK, n0);
+          }
+        }
+        tc::tma_load_2d(w + kOps * kBytesW, &g.map_x, &full[s], kb * kBlockK, 0);
+      }
+    }
+  } else if (warp == 5) {
+    if (lane == 0) {
+      const uint32_t idesc = tc::idesc_f16(Fmt<T>::value, kStreamFeatures, g.cols, 0, g.w_mn);
+      const uint32_t kstep_w = g.w_mn ? 2048 : 32;
+      const uint32_t lbo_w = g.w_mn ? 8192 : 16;
+      for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {
+        const int s = it % g.stages;
+        if (!tc::mbar_wait(&full[s], (it / g.stages) & 1, kWaitLimit)) {
+          ok = false;
+          break;
+        }
+        tc::tc_fence_after();
+        const uint32_t w = tc::smem_u32(smem + s * g.stage_bytes);
+        const uint32_t x = w + kOps * kBytesW;
+#pragma unroll
+        for (int ks = 0; ks < kBlockK / 16; ++ks)
+#pragma unroll
+          for (int op = 0; op < kOps; ++op)
+            tc::mma_f16_ss(tmem + op * kStreamRows,
+                           tc::smem_desc_sw128(w + op * kBytesW + ks * kstep_w, lbo_w, 1024),
+                           tc::smem_desc_sw128(x + ks * 32, 16, 1024), idesc, it > 0 || ks > 0);
+        tc::mma_commit(&empty[s]);
+      }
+      if (ok) tc::mma_commit(&acc_full);
+    }
+  }
+  __syncwarp();
+  const int feature = warp < 4 ? n0 + static_cast<int>(threadIdx.x) : p.outer;
+  const uint32_t taddr = tmem + (static_cast<uint32_t>(warp & 3) << 21);
+  float bias = 0.f;
+  if (kKind == kLinear && p.bias != nullptr && feature < p.outer)
+    bias = to_f32<T>(static_cast<const T*>(p.bias)[feature]);
+  auto finish = [&](int row, float y, float up) {
+    if (kKind == kGated) {
+      y = activate<false>(p.act, y) * up;
+    } else {
+      y = activate<false>(p.act, y + bias);
+      if (p.residual != nullptr)
+        y += to_f32<T>(static_cast<const T*>(p.residual)[row * p.r_rs + feature]);
+    }
+    static_cast<T*>(p.out)[row * p.o_rs + feature] = from_f32<T>(y);
+  };
+  if (warp < 4) {
+    ok = __all_sync(kFullMask, tc::mbar_wait(&acc_full, 0, kWaitLimit));
+    tc::tc_fence_after();
+    if (ok) {
+      float* sums = reinterpret_cast<float*>(smem);  // [op][row][feature], where the stages were
+      for (int c = 0; c < p.rows; c += 16) {
+        uint32_t v[16], up[16];
+        __syncwarp();
+        tc::tmem_ld16(taddr + c, v);
+        if constexpr (kKind == kGated) tc::tmem_ld16(taddr + kStreamRows + c, up);
+        tc::tmem_ld_wait(v);
+        if constexpr (kKind == kGated) tc::tmem_ld_wait(up);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          if (c + j >= p.rows) break;
+          const float y = __uint_as_float(v[j]);
+          const float u = kKind == kGated ? __uint_as_float(up[j]) : 0.f;
+          if (g.splits == 1) {
+            if (feature < p.outer) finish(c + j, y, u);
+          } else {
+            sums[(c + j) * kStreamFeatures + threadIdx.x] = y;
+            if (kKind == kGated) sums[(g.cols + c + j) * kStreamFeatures + threadIdx.x] = u;
+          }
+        }
+      }
+    }
+  }
+  if (!ok) {  // a wait ran out: let copies in flight land before the memory goes
+    aborted = 1;
+    const long long start = clock64();
+    while (clock64() - start < 4000000LL) {
+    }
+  }
+  __syncwarp();
+  if (g.splits > 1) {
+    tc::cluster_sync();
+    // each CTA of the cluster finishes every splits-th row, adding in rank order
+    if (warp < 4 && feature < p.outer) {
+      const float* mine = reinterpret_cast<const float*>(smem) + threadIdx.x;
+      for (int row = rank; row < p.rows; row += g.splits) {
+        float v[8], u[8];
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+          if (s >= g.splits) break;
+          v[s] = tc::ld_peer(tc::peer_smem(mine + row * kStreamFeatures, s));
+          if (kKind == kGated)
+            u[s] = tc::ld_peer(tc::peer_smem(mine + (g.cols + row) * kStreamFeatures, s));
+        }
+        float y = 0.f, up = 0.f;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+          if (s >= g.splits) break;
+          y += v[s];
+          if (kKind == kGated) up += u[s];
+        }
+        finish(row, y, up);
+      }
+    }
+    __syncwarp();
+    tc::tc_fence_before();
+    tc::cluster_sync();  // a peer may still be reading this CTA's sums
+  } else {
+    tc::tc_fence_before();
+    __syncthreads();
+  }
+  if (aborted && threadIdx.x == 0) raise_status(p.status, kStatusTimeout);
+  if (warp == 5) {
+    tc::tc_fence_after();
+    tc::tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
 // ---- host side --------------------------------------------------------------
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -409,6 +607,59 @@ int choose_set(int outer, int row_tiles, int widest, int step, int ctas) {
   return best;
 }
 
+template <typename T, Kind kKind>
+int launch_stream(const StreamParams& g, int tiles, cudaStream_t stream) {
+  constexpr auto kernel = stream_kernel<T, kKind>;
+  if (const cudaError_t e = allow_smem<kernel>(kSmemBudget + 1024)) return static_cast<int>(e);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * g.splits));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = g.stages * g.stage_bytes + 1024;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = g.splits;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return launch_status(cudaLaunchKernelEx(&cfg, kernel, g));
+}
+
+int run_stream(Kind kind, const Problem& p, int32_t dtype, int ctas, cudaStream_t stream) {
+  StreamParams g{};
+  const int ops = kind == kGated ? 2 : 1;
+  g.p = p;
+  g.w_mn = p.w_ks != 1;
+  g.cols = ceil_div(p.rows, 16) * 16;
+  g.stage_bytes = ops * kStreamFeatures * kBlockK * 2 + g.cols * 128;
+  const int tiles = ceil_div(p.outer, kStreamFeatures);
+  const int kblocks = ceil_div(p.inner, kBlockK);
+  // a cluster wide enough that the CTAs fill the SMs about twice
+  g.splits = 1;
+  while (g.splits < 8 && g.splits < kblocks && tiles * (g.splits + 1) <= 2 * ctas) ++g.splits;
+  const int share = ceil_div(kblocks, g.splits);
+  // one CTA per SM may hold the whole ring's budget, two half of it each
+  const int budget = tiles * g.splits <= ctas ? kSmemBudget : 104 * 1024;
+  g.stages = budget / g.stage_bytes;
+  if (g.stages > kStreamStages) g.stages = kStreamStages;
+  if (g.stages > share) g.stages = share;
+  const int sums = ops * g.cols * kStreamFeatures * 4;  // partial sums lie where the stages were
+  while (g.splits > 1 && g.stages * g.stage_bytes < sums) ++g.stages;
+  bool ok = encode2d(&g.map_x, dtype, p.x, p.inner, p.rows, p.x_rs, g.cols);
+  for (int op = 0; op < ops; ++op) {
+    CUtensorMap* map = op ? &g.map_up : &g.map_w;
+    const void* base = op ? p.w_up : p.w;
+    ok = ok && (g.w_mn ? encode2d(map, dtype, base, p.outer, p.inner, p.w_ks, 64)
+                       : encode2d(map, dtype, base, p.inner, p.outer, p.w_ns, kStreamFeatures));
+  }
+  if (!ok) return RLT_E_DEVICE;
+  if (kind == kGated)
+    return dtype == RLT_BF16 ? launch_stream<__nv_bfloat16, kGated>(g, tiles, stream)
+                             : launch_stream<__half, kGated>(g, tiles, stream);
+  return dtype == RLT_BF16 ? launch_stream<__nv_bfloat16, kLinear>(g, tiles, stream)
+                           : launch_stream<__half, kLinear>(g, tiles, stream);
+}
+
 }  // namespace
 
 int tc_vocab_tile(const Problem& p, int ctas) {
@@ -417,6 +668,7 @@ int tc_vocab_tile(const Problem& p, int ctas) {
 }
 
 int run_tc(Kind kind, const Problem& p, int32_t dtype, int ctas, cudaStream_t stream) {
+  if (kind != kVocab && p.rows <= kStreamRows) return run_stream(kind, p, dtype, ctas, stream);
   GemmParams g{};
   g.p = p;
   g.w_mn = p.w_ks != 1;
