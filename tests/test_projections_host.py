@@ -87,11 +87,14 @@ def test_head_arguments():
 
 
 def test_weight_layouts():
-    strides = projections._weight_strides
-    assert strides(torch.zeros(4, 8), "") == (8, 1)
-    assert strides(torch.zeros(8, 4).t(), "") == (1, 4)
-    assert strides(torch.zeros(4, 16)[:, ::16], "") == (16, 1)  # one input feature
-    assert strides(torch.zeros(1, 16)[:, ::2], "") == (1, 2)  # one output feature
+    def strides(w):
+        w = FakeCuda(w)
+        return projections._operands(fake(2, w.shape[1], dtype=w.dtype), w, "")[4:6]
+
+    assert strides(torch.zeros(4, 8)) == (8, 1)
+    assert strides(torch.zeros(8, 4).t()) == (1, 4)
+    assert strides(torch.zeros(4, 16)[:, ::16]) == (16, 1)  # one input feature
+    assert strides(torch.zeros(1, 16)[:, ::2]) == (1, 2)  # one output feature
 
 
 def test_c_entries_refuse_before_any_launch():

@@ -333,6 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
 constexpr int kStreamRows = 64;     // activation rows that stream_kernel takes
 constexpr int kStreamStages = 12;
 constexpr int kStreamFeatures = 128;
+constexpr int kMaxSplits = 8;       // CTAs of a cluster (the portable limit)
 
 struct StreamParams {
   CUtensorMap map_x, map_w, map_up;
@@ -342,9 +343,10 @@ struct StreamParams {
   int cols;    // activation rows rounded up to the instruction's 16
   int w_mn;
   int splits;  // CTAs per feature tile
+  int vec;     // four neighbouring outputs are one 8-byte store
 };
 
-template <typename T, Kind kKind>
+template <typename T, Kind kKind, int kAct>
 __global__ void __launch_bounds__(kThreads) stream_kernel(const __grid_constant__ StreamParams g) {
   constexpr int kOps = kKind == kGated ? 2 : 1;
   constexpr int kBytesW = kStreamFeatures * kBlockK * 2;
@@ -433,45 +435,22 @@ __global__ void __launch_bounds__(kThreads) stream_kernel(const __grid_constant_
     }
   }
   __syncwarp();
-  const int feature = warp < 4 ? n0 + static_cast<int>(threadIdx.x) : p.outer;
-  const uint32_t taddr = tmem + (static_cast<uint32_t>(warp & 3) << 21);
-  float bias = 0.f;
-  if (kKind == kLinear && p.bias != nullptr && feature < p.outer)
-    bias = to_f32<T>(static_cast<const T*>(p.bias)[feature]);
-  auto finish = [&](int row, float y, float up) {
-    if (kKind == kGated) {
-      y = activate<false>(p.act, y) * up;
-    } else {
-      y = activate<false>(p.act, y + bias);
-      if (p.residual != nullptr)
-        y += to_f32<T>(static_cast<const T*>(p.residual)[row * p.r_rs + feature]);
-    }
-    static_cast<T*>(p.out)[row * p.o_rs + feature] = from_f32<T>(y);
-  };
+  float* sums = reinterpret_cast<float*>(smem);  // [op][row][feature], where the stages were
   if (warp < 4) {
     ok = __all_sync(kFullMask, tc::mbar_wait(&acc_full, 0, kWaitLimit));
     tc::tc_fence_after();
-    if (ok) {
-      float* sums = reinterpret_cast<float*>(smem);  // [op][row][feature], where the stages were
-      for (int c = 0; c < p.rows; c += 16) {
-        uint32_t v[16], up[16];
-        __syncwarp();
-        tc::tmem_ld16(taddr + c, v);
-        if constexpr (kKind == kGated) tc::tmem_ld16(taddr + kStreamRows + c, up);
-        tc::tmem_ld_wait(v);
-        if constexpr (kKind == kGated) tc::tmem_ld_wait(up);
+    const uint32_t taddr = tmem + (static_cast<uint32_t>(warp) << 21);
+    for (int c = 0; ok && c < p.rows; c += 16) {
+      float* at = sums + c * kStreamFeatures + threadIdx.x;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          if (c + j >= p.rows) break;
-          const float y = __uint_as_float(v[j]);
-          const float u = kKind == kGated ? __uint_as_float(up[j]) : 0.f;
-          if (g.splits == 1) {
-            if (feature < p.outer) finish(c + j, y, u);
-          } else {
-            sums[(c + j) * kStreamFeatures + threadIdx.x] = y;
-            if (kKind == kGated) sums[(g.cols + c + j) * kStreamFeatures + threadIdx.x] = u;
-          }
-        }
+      for (int op = 0; op < kOps; ++op) {
+        uint32_t v[16];
+        __syncwarp();
+        tc::tmem_ld16(taddr + op * kStreamRows + c, v);
+        tc::tmem_ld_wait(v);
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          at[(op * g.cols + j) * kStreamFeatures] = __uint_as_float(v[j]);
       }
     }
   }
@@ -482,41 +461,78 @@ __global__ void __launch_bounds__(kThreads) stream_kernel(const __grid_constant_
     }
   }
   __syncwarp();
-  if (g.splits > 1) {
+  tc::tc_fence_before();
+  if (g.splits > 1)
     tc::cluster_sync();
-    // each CTA of the cluster finishes every splits-th row, adding in rank order
-    if (warp < 4 && feature < p.outer) {
-      const float* mine = reinterpret_cast<const float*>(smem) + threadIdx.x;
-      for (int row = rank; row < p.rows; row += g.splits) {
-        float v[8], u[8];
-#pragma unroll
-        for (int s = 0; s < 8; ++s) {
-          if (s >= g.splits) break;
-          v[s] = tc::ld_peer(tc::peer_smem(mine + row * kStreamFeatures, s));
-          if (kKind == kGated)
-            u[s] = tc::ld_peer(tc::peer_smem(mine + (g.cols + row) * kStreamFeatures, s));
-        }
-        float y = 0.f, up = 0.f;
-#pragma unroll
-        for (int s = 0; s < 8; ++s) {
-          if (s >= g.splits) break;
-          y += v[s];
-          if (kKind == kGated) up += u[s];
-        }
-        finish(row, y, up);
-      }
-    }
-    __syncwarp();
-    tc::tc_fence_before();
-    tc::cluster_sync();  // a peer may still be reading this CTA's sums
-  } else {
-    tc::tc_fence_before();
+  else
     __syncthreads();
-  }
   if (aborted && threadIdx.x == 0) raise_status(p.status, kStatusTimeout);
   if (warp == 5) {
     tc::tc_fence_after();
     tc::tmem_dealloc(tmem, kTmemCols);
+  }
+  // Each CTA of the cluster finishes every splits-th row, adding in rank order:
+  // a warp per row, four neighbouring features per lane.
+  const int f0 = lane * 4;
+  const int n = n0 + f0;
+  if (n < p.outer) {
+    const T* res = static_cast<const T*>(p.residual);
+    float b[4] = {0.f, 0.f, 0.f, 0.f};
+    if (kKind == kLinear && p.bias != nullptr)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n + e < p.outer) b[e] = to_f32<T>(static_cast<const T*>(p.bias)[n + e]);
+#pragma unroll 2
+    for (int row = rank + warp * g.splits; row < p.rows; row += kThreads / 32 * g.splits) {
+      float r[4] = {0.f, 0.f, 0.f, 0.f};
+      if (kKind == kLinear && res != nullptr)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n + e < p.outer) r[e] = to_f32<T>(res[row * p.r_rs + n + e]);
+      float y[kOps][4];
+#pragma unroll
+      for (int op = 0; op < kOps; ++op) {
+        const float* mine = sums + (op * g.cols + row) * kStreamFeatures + f0;
+        float4 v[kMaxSplits];
+#pragma unroll
+        for (int s = 0; s < kMaxSplits; ++s)
+          if (s < g.splits) v[s] = g.splits > 1 ? tc::ld_peer4(tc::peer_smem(mine, s))
+                                                : *reinterpret_cast<const float4*>(mine);
+        float4 t = v[0];
+#pragma unroll
+        for (int s = 1; s < kMaxSplits; ++s)
+          if (s < g.splits) {
+            t.x += v[s].x;
+            t.y += v[s].y;
+            t.z += v[s].z;
+            t.w += v[s].w;
+          }
+        y[op][0] = t.x;
+        y[op][1] = t.y;
+        y[op][2] = t.z;
+        y[op][3] = t.w;
+      }
+      T o[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (kKind == kGated)
+          o[e] = from_f32<T>(activate<false, kAct>(y[0][e]) * y[1][e]);
+        else
+          o[e] = from_f32<T>(activate<false, kAct>(y[0][e] + b[e]) + r[e]);
+      }
+      T* out = static_cast<T*>(p.out) + row * p.o_rs + n;
+      if (g.vec) {
+        *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(o);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n + e < p.outer) out[e] = o[e];
+      }
+    }
+  }
+  if (g.splits > 1) {
+    __syncwarp();
+    tc::cluster_sync();  // a peer may still be reading this CTA's sums
   }
 }
 
@@ -567,24 +583,11 @@ cudaError_t allow_smem(int bytes) {
 }
 
 template <typename T, Kind kKind, int kAct>
-int launch_gemm(const GemmParams& g, int ctas, cudaStream_t stream) {
+int launch(const GemmParams& g, int ctas, cudaStream_t stream) {
   constexpr auto kernel = gemm_kernel<T, kKind, kAct>;
   if (const cudaError_t e = allow_smem<kernel>(kSmemBudget + 1024)) return static_cast<int>(e);
   kernel<<<ctas, kThreads, g.stages * g.stage_bytes + 1024, stream>>>(g);
   return launch_status(cudaGetLastError());
-}
-
-template <typename T, Kind kKind>
-int launch_act(const GemmParams& g, int ctas, cudaStream_t stream) {
-  if constexpr (kKind == kVocab) return launch_gemm<T, kKind, RLT_ACT_NONE>(g, ctas, stream);
-  switch (g.p.act) {
-    case RLT_ACT_SILU: return launch_gemm<T, kKind, RLT_ACT_SILU>(g, ctas, stream);
-    case RLT_ACT_GELU: return launch_gemm<T, kKind, RLT_ACT_GELU>(g, ctas, stream);
-    case RLT_ACT_GELU_TANH: return launch_gemm<T, kKind, RLT_ACT_GELU_TANH>(g, ctas, stream);
-    case RLT_ACT_RELU: return launch_gemm<T, kKind, RLT_ACT_RELU>(g, ctas, stream);
-    case RLT_ACT_SIGMOID: return launch_gemm<T, kKind, RLT_ACT_SIGMOID>(g, ctas, stream);
-    default: return launch_gemm<T, kKind, RLT_ACT_NONE>(g, ctas, stream);
-  }
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -607,9 +610,9 @@ int choose_set(int outer, int row_tiles, int widest, int step, int ctas) {
   return best;
 }
 
-template <typename T, Kind kKind>
-int launch_stream(const StreamParams& g, int tiles, cudaStream_t stream) {
-  constexpr auto kernel = stream_kernel<T, kKind>;
+template <typename T, Kind kKind, int kAct>
+int launch(const StreamParams& g, int tiles, cudaStream_t stream) {
+  constexpr auto kernel = stream_kernel<T, kKind, kAct>;
   if (const cudaError_t e = allow_smem<kernel>(kSmemBudget + 1024)) return static_cast<int>(e);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(tiles * g.splits));
@@ -625,26 +628,46 @@ int launch_stream(const StreamParams& g, int tiles, cudaStream_t stream) {
   return launch_status(cudaLaunchKernelEx(&cfg, kernel, g));
 }
 
+// The kernel for a launch's type and activation.
+template <Kind kKind, typename T, typename Params>
+int by_activation(const Params& g, int ctas, cudaStream_t stream) {
+  if constexpr (kKind == kVocab) return launch<T, kKind, RLT_ACT_NONE>(g, ctas, stream);
+  switch (g.p.act) {
+    case RLT_ACT_SILU: return launch<T, kKind, RLT_ACT_SILU>(g, ctas, stream);
+    case RLT_ACT_GELU: return launch<T, kKind, RLT_ACT_GELU>(g, ctas, stream);
+    case RLT_ACT_GELU_TANH: return launch<T, kKind, RLT_ACT_GELU_TANH>(g, ctas, stream);
+    case RLT_ACT_RELU: return launch<T, kKind, RLT_ACT_RELU>(g, ctas, stream);
+    case RLT_ACT_SIGMOID: return launch<T, kKind, RLT_ACT_SIGMOID>(g, ctas, stream);
+    default: return launch<T, kKind, RLT_ACT_NONE>(g, ctas, stream);
+  }
+}
+template <Kind kKind, typename Params>
+int by_type(const Params& g, int32_t dtype, int ctas, cudaStream_t stream) {
+  return dtype == RLT_BF16 ? by_activation<kKind, __nv_bfloat16>(g, ctas, stream)
+                           : by_activation<kKind, __half>(g, ctas, stream);
+}
+
 int run_stream(Kind kind, const Problem& p, int32_t dtype, int ctas, cudaStream_t stream) {
   StreamParams g{};
   const int ops = kind == kGated ? 2 : 1;
   g.p = p;
   g.w_mn = p.w_ks != 1;
   g.cols = ceil_div(p.rows, 16) * 16;
+  g.vec = p.outer % 4 == 0 && p.o_rs % 4 == 0 && reinterpret_cast<uintptr_t>(p.out) % 8 == 0;
   g.stage_bytes = ops * kStreamFeatures * kBlockK * 2 + g.cols * 128;
   const int tiles = ceil_div(p.outer, kStreamFeatures);
   const int kblocks = ceil_div(p.inner, kBlockK);
   // a cluster wide enough that the CTAs fill the SMs about twice
   g.splits = 1;
-  while (g.splits < 8 && g.splits < kblocks && tiles * (g.splits + 1) <= 2 * ctas) ++g.splits;
+  while (g.splits < kMaxSplits && g.splits < kblocks && tiles * (g.splits + 1) <= 2 * ctas) ++g.splits;
   const int share = ceil_div(kblocks, g.splits);
-  // one CTA per SM may hold the whole ring's budget, two half of it each
-  const int budget = tiles * g.splits <= ctas ? kSmemBudget : 104 * 1024;
-  g.stages = budget / g.stage_bytes;
+  // two CTAs fit an SM, so that a cluster finds room whatever the number of
+  // SMs its part of the die has
+  g.stages = 110 * 1024 / g.stage_bytes;
   if (g.stages > kStreamStages) g.stages = kStreamStages;
   if (g.stages > share) g.stages = share;
   const int sums = ops * g.cols * kStreamFeatures * 4;  // partial sums lie where the stages were
-  while (g.splits > 1 && g.stages * g.stage_bytes < sums) ++g.stages;
+  while (g.stages * g.stage_bytes < sums) ++g.stages;
   bool ok = encode2d(&g.map_x, dtype, p.x, p.inner, p.rows, p.x_rs, g.cols);
   for (int op = 0; op < ops; ++op) {
     CUtensorMap* map = op ? &g.map_up : &g.map_w;
@@ -653,11 +676,8 @@ int run_stream(Kind kind, const Problem& p, int32_t dtype, int ctas, cudaStream_
                        : encode2d(map, dtype, base, p.inner, p.outer, p.w_ns, kStreamFeatures));
   }
   if (!ok) return RLT_E_DEVICE;
-  if (kind == kGated)
-    return dtype == RLT_BF16 ? launch_stream<__nv_bfloat16, kGated>(g, tiles, stream)
-                             : launch_stream<__half, kGated>(g, tiles, stream);
-  return dtype == RLT_BF16 ? launch_stream<__nv_bfloat16, kLinear>(g, tiles, stream)
-                           : launch_stream<__half, kLinear>(g, tiles, stream);
+  return kind == kGated ? by_type<kGated>(g, dtype, tiles, stream)
+                        : by_type<kLinear>(g, dtype, tiles, stream);
 }
 
 }  // namespace
@@ -695,15 +715,11 @@ int run_tc(Kind kind, const Problem& p, int32_t dtype, int ctas, cudaStream_t st
   if (!ok) return RLT_E_DEVICE;
   const int tiles = g.row_tiles * g.col_tiles;
   if (tiles < ctas) ctas = tiles;
-#define RLT_TC(KIND)                                                         \
-  (dtype == RLT_BF16 ? launch_act<__nv_bfloat16, KIND>(g, ctas, stream)      \
-                     : launch_act<__half, KIND>(g, ctas, stream))
   switch (kind) {
-    case kLinear: return RLT_TC(kLinear);
-    case kGated: return RLT_TC(kGated);
-    default: return RLT_TC(kVocab);
+    case kLinear: return by_type<kLinear>(g, dtype, ctas, stream);
+    case kGated: return by_type<kGated>(g, dtype, ctas, stream);
+    default: return by_type<kVocab>(g, dtype, ctas, stream);
   }
-#undef RLT_TC
 }
 
 }  // namespace proj

@@ -25,28 +25,35 @@ ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2, "gelu_tanh": 3, "relu": 4, "sigmoi
 
 
 def _operands(x, weight, what):
-    """Check x [rows, in] and weight [out, in]; returns x with contiguous rows."""
-    if x.ndim != 2 or weight.ndim != 2 or x.shape[1] != weight.shape[1]:
+    """Check x [rows, in] and weight [out, in]; returns x with contiguous rows,
+    rows, in, out, the weight's strides (one of them 1) and the dtype's code."""
+    try:
+        rows, inner = x.shape
+        outer, inner_w = weight.shape
+    except ValueError:
+        inner, inner_w = 0, -1
+    if inner != inner_w:
         raise ValueError(f"{what}: expected x [rows, in] and weight [out, in]")
-    if x.device.type != "cuda":
+    device, dtype = x.device, x.dtype
+    if device.type != "cuda":
         raise ValueError(f"{what} requires a CUDA device")
-    if x.dtype not in _lib.DTYPE_CODES or weight.dtype != x.dtype:
+    code = _lib.DTYPE_CODES.get(dtype)
+    if code is None or weight.dtype != dtype:
         raise ValueError(f"{what}: x and weight must share a float32, float16 or bfloat16 dtype")
-    if weight.device != x.device:
+    if weight.device != device:
         raise ValueError(f"{what}: all tensors must live on the same device")
-    if x.shape[1] == 0:
+    if inner == 0:
         raise ValueError(f"{what}: in_features must be positive")
-    return x if x.stride(1) == 1 else x.contiguous()
-
-
-def _weight_strides(weight, what):
-    """(between output features, between input features), one of them 1."""
     ns, ks = weight.stride()
-    if ks == 1 or weight.shape[1] == 1:
-        return ns, 1
-    if ns == 1 or weight.shape[0] == 1:
-        return 1, ks
-    raise ValueError(f"{what}: one dimension of weight must be contiguous")
+    if ks == 1 or inner == 1:
+        ks = 1
+    elif ns == 1 or outer == 1:
+        ns = 1
+    else:
+        raise ValueError(f"{what}: one dimension of weight must be contiguous")
+    if x.stride(1) != 1:
+        x = x.contiguous()
+    return x, rows, inner, outer, ns, ks, code
 
 
 def _rows_like(t, x, outer, name, what):
@@ -54,11 +61,11 @@ def _rows_like(t, x, outer, name, what):
         raise ValueError(f"{what}: {name} must be [rows, out] of x's dtype and device")
 
 
-def _output(out, x, outer, what):
+def _output(out, x, rows, outer, what):
     if out is None:
-        return torch.empty((x.shape[0], outer), device=x.device, dtype=x.dtype)
+        return x.new_empty((rows, outer))
     _rows_like(out, x, outer, "out", what)
-    if outer > 1 and out.stride(1) != 1 or x.shape[0] > 1 and out.stride(0) < outer:
+    if outer > 1 and out.stride(1) != 1 or rows > 1 and out.stride(0) < outer:
         raise ValueError(f"{what}: rows of out must be contiguous and apart")
     return out
 
@@ -70,8 +77,22 @@ def _activation(name, what):
         raise ValueError(f"{what}: activation must be one of {list(ACTIVATIONS)}") from None
 
 
-def _scratch(need, device):
-    return torch.empty(need, dtype=torch.uint8, device=device) if need else None
+def _run(device, what, entry, need, *args):
+    """Call ``entry(workspace, bytes, status, stream)`` on ``device``; scratch
+    is only asked for, and allocated, by the few calls whose operands have to be
+    copied into aligned rows (they are refused without it)."""
+    index = device.index
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _run(device, what, entry, need, *args)
+    status, stream = _lib.status_word(device).data_ptr(), _lib.stream_of(device)
+    rc = entry(None, 0, status, stream)
+    if rc == _lib.E_WORKSPACE:
+        size = need(*args)
+        scratch = torch.empty(size, dtype=torch.uint8, device=device)
+        rc = entry(scratch.data_ptr(), size, status, stream)
+    if rc:
+        _lib.check(rc, what)
 
 
 def linear(x, weight, bias=None, *, activation=None, residual=None, out=None):
@@ -82,33 +103,30 @@ def linear(x, weight, bias=None, *, activation=None, residual=None, out=None):
     "gelu_tanh", "relu" or "sigmoid". ``out`` may be ``residual`` itself and
     must not overlap any other argument."""
     what = "linear"
-    x = _operands(x, weight, what)
-    rows, inner = x.shape
-    outer = weight.shape[0]
+    x, rows, inner, outer, ns, ks, code = _operands(x, weight, what)
     act = _activation(activation, what)
-    ns, ks = _weight_strides(weight, what)
+    bias_ptr = residual_ptr = None
+    residual_stride = 0
     if bias is not None:
         if bias.shape != (outer,) or bias.dtype != x.dtype or bias.device != x.device:
             raise ValueError(f"{what}: bias must be [out] of x's dtype and device")
         bias = bias.contiguous()
+        bias_ptr = bias.data_ptr()
     if residual is not None:
         _rows_like(residual, x, outer, "residual", what)
         if residual.stride(1) != 1:
             residual = residual.contiguous()
-    result = _output(out, x, outer, what)
+        residual_ptr, residual_stride = residual.data_ptr(), residual.stride(0)
+    result = _output(out, x, rows, outer, what)
     if rows == 0 or outer == 0:
         return result
-    lib, device, code = _lib.load(), x.device, _lib.DTYPE_CODES[x.dtype]
-    with torch.cuda.device(device):
-        xp, wp, xs = x.data_ptr(), weight.data_ptr(), x.stride(0)
-        need = lib.rlt_linear_workspace_bytes(xp, wp, code, rows, inner, outer, 0, xs, ns, ks)
-        scratch = _scratch(need, device)
-        rc = lib.rlt_linear(
-            xp, wp, _lib.ptr(bias), _lib.ptr(residual), result.data_ptr(), _lib.ptr(scratch), need,
-            _lib.status_word(device).data_ptr(), code, rows, inner, outer, act, xs, ns, ks,
-            0 if residual is None else residual.stride(0), result.stride(0),
-            _lib.stream_of(device))
-    _lib.check(rc, what)
+    lib, xp, wp, xs = _lib.load(), x.data_ptr(), weight.data_ptr(), x.stride(0)
+    op, os = result.data_ptr(), result.stride(0)
+    _run(x.device, what,
+         lambda scratch, size, status, stream: lib.rlt_linear(
+             xp, wp, bias_ptr, residual_ptr, op, scratch, size, status, code, rows, inner, outer,
+             act, xs, ns, ks, residual_stride, os, stream),
+         lib.rlt_linear_workspace_bytes, xp, wp, code, rows, inner, outer, 0, xs, ns, ks)
     return result
 
 
@@ -116,53 +134,45 @@ def gated_linear(x, weight, *, activation="silu", out=None):
     """``act(x @ gate.t()) * (x @ up.t())`` in one kernel, ``weight`` being
     ``[gate; up]``, ``[2 * features, in]``. Returns ``[rows, features]``."""
     what = "gated linear"
-    x = _operands(x, weight, what)
-    if weight.shape[0] % 2:
+    x, rows, inner, outer, ns, ks, code = _operands(x, weight, what)
+    if outer % 2:
         raise ValueError(f"{what}: weight must hold as many gate rows as up rows")
-    rows, inner = x.shape
-    outer = weight.shape[0] // 2
+    outer //= 2
     act = _activation(activation, what)
-    ns, ks = _weight_strides(weight, what)
-    result = _output(out, x, outer, what)
+    result = _output(out, x, rows, outer, what)
     if rows == 0 or outer == 0:
         return result
-    lib, device, code = _lib.load(), x.device, _lib.DTYPE_CODES[x.dtype]
-    with torch.cuda.device(device):
-        xp, wp, xs = x.data_ptr(), weight.data_ptr(), x.stride(0)
-        need = lib.rlt_linear_workspace_bytes(xp, wp, code, rows, inner, outer, 1, xs, ns, ks)
-        scratch = _scratch(need, device)
-        rc = lib.rlt_gated_linear(
-            xp, wp, result.data_ptr(), _lib.ptr(scratch), need,
-            _lib.status_word(device).data_ptr(), code, rows, inner, outer, act, xs, ns, ks,
-            result.stride(0), _lib.stream_of(device))
-    _lib.check(rc, what)
+    lib, xp, wp, xs = _lib.load(), x.data_ptr(), weight.data_ptr(), x.stride(0)
+    op, os = result.data_ptr(), result.stride(0)
+    _run(x.device, what,
+         lambda scratch, size, status, stream: lib.rlt_gated_linear(
+             xp, wp, op, scratch, size, status, code, rows, inner, outer, act, xs, ns, ks, os,
+             stream),
+         lib.rlt_linear_workspace_bytes, xp, wp, code, rows, inner, outer, 1, xs, ns, ks)
     return result
 
 
 def _vocab_head(hidden, weight, tokens, what):
-    hidden = _operands(hidden, weight, what)
-    rows, inner = hidden.shape
-    vocab = weight.shape[0]
+    hidden, rows, inner, vocab, ns, ks, code = _operands(hidden, weight, what)
     if vocab == 0:
         raise ValueError(f"{what}: the vocabulary must not be empty")
-    ns, ks = _weight_strides(weight, what)
     device = hidden.device
-    chosen = None
+    chosen = chosen_ptr = tokens_ptr = None
     if tokens is None:
         chosen = torch.empty(rows, dtype=torch.int64, device=device)
+        chosen_ptr = chosen.data_ptr()
+    else:
+        tokens_ptr = tokens.data_ptr()
     logprobs = torch.empty(rows, dtype=torch.float32, device=device)
     if rows == 0:
         return chosen, logprobs
-    lib, code = _lib.load(), _lib.DTYPE_CODES[hidden.dtype]
-    with torch.cuda.device(device):
-        hp, wp, hs = hidden.data_ptr(), weight.data_ptr(), hidden.stride(0)
-        need = lib.rlt_vocab_head_workspace_bytes(hp, wp, code, rows, inner, vocab, hs, ns, ks)
-        scratch = _scratch(need, device)
-        rc = lib.rlt_vocab_head(
-            hp, wp, _lib.ptr(tokens), _lib.ptr(chosen), logprobs.data_ptr(), _lib.ptr(scratch),
-            need, _lib.status_word(device).data_ptr(), code, rows, inner, vocab, hs, ns, ks,
-            _lib.stream_of(device))
-    _lib.check(rc, what)
+    lib, hp, wp, hs = _lib.load(), hidden.data_ptr(), weight.data_ptr(), hidden.stride(0)
+    lp = logprobs.data_ptr()
+    _run(device, what,
+         lambda scratch, size, status, stream: lib.rlt_vocab_head(
+             hp, wp, tokens_ptr, chosen_ptr, lp, scratch, size, status, code, rows, inner, vocab,
+             hs, ns, ks, stream),
+         lib.rlt_vocab_head_workspace_bytes, hp, wp, code, rows, inner, vocab, hs, ns, ks)
     return chosen, logprobs
 
 
