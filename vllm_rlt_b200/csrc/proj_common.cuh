@@ -107,7 +107,8 @@ __device__ __forceinline__ void fold(VocabPart& a, const VocabPart& b) {
 
 // Tensor-core path (16-bit operands whose pointers and strides TMA accepts).
 int run_tc(Kind kind, const Problem& p, int32_t dtype, int ctas, cudaStream_t stream);
-int tc_vocab_tile(const Problem& p, int ctas);
+// Vocabulary records per row that it leaves.
+int tc_vocab_parts(const Problem& p, int ctas);
 
 }  // namespace proj
 }  // namespace rlt

@@ -418,10 +418,10 @@ int dispatch(Problem p, int32_t dtype, char* copies, cudaStream_t stream) {
   return run_tc(kKind, p, dtype, sm_count(), stream);
 }
 
-// Columns per vocabulary tile of the kernel that the call will run.
-int vocab_tile(const Problem& p, int32_t dtype) {
-  if (dtype != RLT_F32) return tc_vocab_tile(p, sm_count());
-  return fma_tile(p.rows, p.outer) == 2 ? 128 : 64;
+// Vocabulary records per row that the call's kernel leaves.
+int vocab_parts(const Problem& p, int32_t dtype) {
+  if (dtype != RLT_F32) return tc_vocab_parts(p, sm_count());
+  return ceil_div(p.outer, fma_tile(p.rows, p.outer) == 2 ? 128 : 64);
 }
 
 bool known(int32_t dtype) { return dtype == RLT_F32 || dtype == RLT_F16 || dtype == RLT_BF16; }
@@ -454,7 +454,7 @@ const void* up_rows(const void* weight, int32_t dtype, int32_t out_features, int
 }
 
 size_t parts_bytes(const Problem& p, int32_t dtype) {
-  return static_cast<size_t>(p.rows) * ceil_div(p.outer, vocab_tile(p, dtype)) * sizeof(VocabPart);
+  return static_cast<size_t>(p.rows) * vocab_parts(p, dtype) * sizeof(VocabPart);
 }
 
 }  // namespace
@@ -562,7 +562,7 @@ extern "C" int rlt_vocab_head(const void* hidden, const void* weight, const int6
   p.status = status;
   p.tokens = tokens;
   p.parts = static_cast<VocabPart*>(workspace);
-  p.tiles = ceil_div(vocab, vocab_tile(p, dtype));
+  p.tiles = vocab_parts(p, dtype);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (const int rc = dispatch<kVocab>(p, dtype, static_cast<char*>(workspace) + parts, s))
     return rc;

@@ -1,13 +1,24 @@
 // Projections on the tensor cores (bf16, fp16; fp32 accumulation in TMEM).
 //
-// gemm_kernel: a CTA takes tiles of 128 activation rows by up to 256 weight
-// rows (output features). One thread of warp 4 copies 64-feature slices of
-// both operands into a ring of shared-memory stages by TMA (128-byte swizzle),
-// one thread of warp 5 issues the tcgen05.mma, and warps 0-3 turn a finished
-// accumulator into outputs while the next tile accumulates in the other half
-// of TMEM. A thread of warps 0-3 owns one activation row of the tile (its TMEM
-// lane) and walks the row's columns, so the vocabulary head's maximum and sum
-// need no exchange between threads.
+// gemm_kernel: tiles of 128 activation rows by up to 256 weight rows (output
+// features), or of 256 by 256 on a pair of CTAs (cta_group::2). A thread of
+// warp 8 copies 64-feature slices of both operands into a ring of
+// shared-memory stages by TMA (128-byte swizzle), one of warp 9 issues the
+// tcgen05.mma, and warps 0-7 turn a finished accumulator into outputs while
+// the next one fills the other half of TMEM.
+//
+// What bounds a tile: 64 input features take 2 N cycles of arithmetic, and an
+// SM takes in about 60 bytes a cycle from L2, (128 + N) x 128 bytes for a CTA
+// by itself, (128 + N / 2) x 128 for one of a pair (each holds half of the
+// weights' slice). At N = 256 that is 819 and 546 cycles against 512, so wide
+// tiles on pairs are the ones near the tensor cores' rate.
+//
+// A thread of warps 0-7 holds one activation row of the tile (its TMEM lane)
+// and half of its columns, so the vocabulary head's maximum and sum need no
+// exchange between threads. The tensor core truncates as it accumulates (an
+// error of one sign that grows with the number of k-steps), so the head, whose
+// outputs are fp32, accumulates at most 512 input features in TMEM and adds
+// those sums in registers, rounded to nearest.
 //
 // Weights may have either dimension contiguous: with the input features
 // contiguous a stage holds them K-major (128-byte rows of 64 input features),
@@ -34,16 +45,24 @@ namespace {
 constexpr long long kWaitLimit = 100000000LL;  // cycles (~50 ms)
 constexpr int kBlockK = 64;                    // input features per stage (128 bytes)
 constexpr int kTileM = 128;                    // activation rows per CTA
-constexpr int kMaxStages = 8;
-constexpr int kThreads = 192;
-constexpr int kBytesA = kTileM * kBlockK * 2;
-constexpr int kSmemBudget = 200 * 1024;
+constexpr int kMaxStages = 10;
+constexpr int kEpilogueWarps = 8;
+// Warps 8 and 9 copy and multiply; 10 and 11 complete their warpgroup. The
+// head's epilogue threads hold 128 sums each and take registers from it.
+constexpr int kThreads = (kEpilogueWarps + 4) * 32;
+constexpr int kLaunchRegs = 168, kSumRegs = 232, kOtherRegs = 40;  // per thread, the head's kernel
+static_assert(256 * kSumRegs + 128 * kOtherRegs <= kThreads * kLaunchRegs,
+              "the increase draws on what the launch allocated");
+constexpr int kStagingBytes = kEpilogueWarps * 4096;  // 32 rows x 32 fp32 columns per warp
+constexpr int kSmemBudget = 224 * 1024;               // dynamic shared memory of a CTA
+constexpr int kVocabBlocks = 8;  // 64-feature blocks accumulated in TMEM at a time by the head
 
 struct GemmParams {
   CUtensorMap map_x, map_w, map_up;
   Problem p;
   int stages;
   int stage_bytes;
+  int ring_bytes;
   int box_m;      // activation rows copied per stage (the rest of the tile is never stored)
   int tile_n;     // accumulator columns: output features, or gate then up features
   int load_n;     // weight rows this CTA copies per operand
@@ -51,7 +70,22 @@ struct GemmParams {
   int w_mn;       // weights MN-major in shared memory
   int row_tiles;
   int col_tiles;
-  int vec;        // out (and bias, residual) allow 16-byte access
+  int vec;        // out (and bias, residual) allow 8-byte access
+  int pair;       // tiles of 256 rows on pairs of CTAs
+};
+
+// Position in a ring of barriers: a slot, and the parity its next use has. The
+// issuing threads step it without divisions (with them a 64-feature block took
+// them 570 and 740 cycles, more than its 512 of arithmetic).
+struct Ring {
+  int slot = 0;
+  uint32_t parity = 0;
+  __device__ __forceinline__ void next(int size) {
+    if (++slot == size) {
+      slot = 0;
+      parity ^= 1;
+    }
+  }
 };
 
 template <typename T>
@@ -65,251 +99,363 @@ struct Fmt<__nv_bfloat16> {
   static constexpr uint32_t value = 1;
 };
 
-// 32 outputs of one row from column n on, up to column `end`: y = act(acc + bias) + residual, or
-// act(acc) * up.
-template <typename T, Kind kKind, int kAct>
-__device__ __forceinline__ void finish32(const Problem& p, int vec, int row, int n, int end,
-                                         const uint32_t (&acc)[32], const uint32_t (&up)[32]) {
+// Four neighbouring 16-bit values (8-byte aligned in memory).
+template <typename T>
+__device__ __forceinline__ void widen4(const uint2& r, float (&v)[4]) {
+  T t[4];
+  *reinterpret_cast<uint2*>(t) = r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = to_f32<T>(t[e]);
+}
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, float (&v)[4]) {
+  widen4<T>(*reinterpret_cast<const uint2*>(p), v);
+}
+
+// Columns n .. n + 31 of a warp's 32 rows, from the threads' registers (one row
+// each) to `out`: the values go through shared memory so that neighbouring
+// lanes hold neighbouring columns, then y = act(v + bias) + residual. 16-byte
+// units are swizzled by row, which keeps both directions free of bank
+// conflicts. `end`: columns that exist.
+template <typename T, int kAct>
+__device__ __forceinline__ void finish32(const Problem& p, int vec, uint8_t* staging, int row0,
+                                         int n, int end, const float (&v)[32]) {
+  const int lane = threadIdx.x & 31;
   const T* bias = static_cast<const T*>(p.bias);
   const T* res = static_cast<const T*>(p.residual);
-  T* out = static_cast<T*>(p.out) + row * p.o_rs + n;
-  if (res != nullptr) res += row * p.r_rs + n;
-  const bool in_row = row < p.rows;
+  T* out = static_cast<T*>(p.out);
+  const int rows = min(32, p.rows - row0);
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    float y[8], b[8], r[8];
-    const bool whole = vec && n + g * 8 + 8 <= end;
-    if (kKind == kLinear && bias != nullptr) {
-      if (whole) {
-        unpack16<T>(ld_vec(bias + n + g * 8), b);
-      } else {
+  for (int c = 0; c < 8; ++c)
+    *reinterpret_cast<float4*>(staging + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+        make_float4(v[c * 4], v[c * 4 + 1], v[c * 4 + 2], v[c * 4 + 3]);
+  if (vec && n + 32 <= end) {  // 8 lanes per row, four columns each
+    const int c = lane & 7, at = n + c * 4;
+    float b[4] = {0.f, 0.f, 0.f, 0.f};
+    uint2 r[8];  // the residuals, on their way together
+    if (bias != nullptr) load4<T>(bias + at, b);
+    if (res != nullptr)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) b[e] = n + g * 8 + e < end ? to_f32<T>(bias[n + g * 8 + e]) : 0.f;
-      }
-    }
-    if (kKind == kLinear && res != nullptr && in_row) {
-      if (whole) {
-        unpack16<T>(ld_vec(res + g * 8), r);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) r[e] = n + g * 8 + e < end ? to_f32<T>(res[g * 8 + e]) : 0.f;
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      y[e] = __uint_as_float(acc[g * 8 + e]);
-      if (kKind == kGated) {
-        y[e] = activate<false, kAct>(y[e]) * __uint_as_float(up[g * 8 + e]);
-      } else {
-        if (bias != nullptr) y[e] += b[e];
-        y[e] = activate<false, kAct>(y[e]);
-        if (res != nullptr && in_row) y[e] += r[e];
-      }
-    }
-    if (!in_row) continue;
-    if (whole) {
-      st_vec(out + g * 8, pack16<T>(y));
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (n + g * 8 + e < end) out[g * 8 + e] = from_f32<T>(y[e]);
-    }
-  }
-}
-
-// A row's record of one vocabulary tile, from the accumulator's columns. The
-// running maximum and sum move chunk by chunk (32 logits in registers).
-__device__ __forceinline__ void vocab_tile_part(const GemmParams& g, uint32_t taddr, int row,
-                                                int n0, int tile) {
-  const Problem& p = g.p;
-  const int cols = min(g.tile_n, p.outer - n0);
-  const bool in_row = row < p.rows;
-  const int64_t want64 = in_row && p.tokens != nullptr ? p.tokens[row] : -1;
-  const int want = want64 >= n0 && want64 < n0 + cols ? static_cast<int>(want64) - n0 : -1;
-  VocabPart part{-INFINITY, 0.f, n0, 0.f};
-  for (int c = 0; c < cols; c += 32) {
-    uint32_t v[32];
+      for (int i = 0; i < 8; ++i)
+        if (i * 4 + (lane >> 3) < rows)
+          r[i] = *reinterpret_cast<const uint2*>(res + (row0 + i * 4 + (lane >> 3)) * p.r_rs + at);
     __syncwarp();
-    tc::tmem_ld32(taddr + c, v);
-    tc::tmem_ld_wait(v);
-    const int left = cols - c;
-    if (left < 32) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (j >= left) v[j] = __float_as_uint(-INFINITY);
+    for (int i = 0; i < 8; ++i) {
+      const int row = i * 4 + (lane >> 3);
+      if (row >= rows) continue;
+      const float4 f =
+          *reinterpret_cast<const float4*>(staging + row * 128 + ((c ^ (row & 7)) << 4));
+      float y[4] = {f.x, f.y, f.z, f.w};
+      float add[4] = {0.f, 0.f, 0.f, 0.f};
+      if (res != nullptr) widen4<T>(r[i], add);
+      T o[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = from_f32<T>(activate<false, kAct>(y[e] + b[e]) + add[e]);
+      *reinterpret_cast<uint2*>(out + (row0 + row) * p.o_rs + at) = *reinterpret_cast<uint2*>(o);
     }
-    float m = __uint_as_float(v[0]);
+  } else {  // one column per lane
+    __syncwarp();
+    if (n + lane < end) {
+      const int at = n + lane;
+      const float b = bias != nullptr ? to_f32<T>(bias[at]) : 0.f;
+      for (int row = 0; row < rows; row += 8) {
+        float y[8];
 #pragma unroll
-    for (int j = 1; j < 32; ++j) m = fmaxf(m, __uint_as_float(v[j]));
-    if (m > part.most) {
-      if (p.tokens == nullptr) {
-        int at = 0;
+        for (int i = 0; i < 8; ++i)
+          y[i] = res != nullptr && row + i < rows ? to_f32<T>(res[(row0 + row + i) * p.r_rs + at])
+                                                  : 0.f;
 #pragma unroll
-        for (int j = 31; j >= 0; --j)
-          if (__uint_as_float(v[j]) == m) at = j;
-        part.at = n0 + c + at;
-      }
-      part.sum *= ex2((part.most - m) * kLog2e);
-      part.most = m;
-    }
-    const float base = part.most == -INFINITY ? 0.f : part.most;
-    float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-    for (int j = 0; j < 32; j += 2) {
-      s0 += ex2((__uint_as_float(v[j]) - base) * kLog2e);
-      s1 += ex2((__uint_as_float(v[j + 1]) - base) * kLog2e);
-    }
-    part.sum += s0 + s1;
-    if (__any_sync(kFullMask, want >= c && want < c + 32)) {
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (want == c + j) part.chosen = __uint_as_float(v[j]);
-    }
-  }
-  // a NaN among the logits counts as the largest: find the first
-  if (p.tokens == nullptr && __any_sync(kFullMask, part.sum != part.sum)) {
-    for (int c = (cols - 1) / 32 * 32; c >= 0; c -= 32) {
-      uint32_t v[32];
-      __syncwarp();
-      tc::tmem_ld32(taddr + c, v);
-      tc::tmem_ld_wait(v);
-#pragma unroll
-      for (int j = 31; j >= 0; --j) {
-        const float l = __uint_as_float(v[j]);
-        if (c + j < cols && l != l) {
-          part.most = l;
-          part.at = n0 + c + j;
+        for (int i = 0; i < 8; ++i) {
+          const float f = *reinterpret_cast<const float*>(
+              staging + (row + i) * 128 + (((lane >> 2) ^ i) << 4) + (lane & 3) * 4);
+          y[i] += activate<false, kAct>(f + b);
         }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (row + i < rows) out[(row0 + row + i) * p.o_rs + at] = from_f32<T>(y[i]);
       }
     }
   }
-  if (in_row) p.parts[static_cast<int64_t>(row) * p.tiles + tile] = part;
+  __syncwarp();
 }
 
-template <typename T, Kind kKind, int kAct>
+// A thread's record of its columns v[0 .. cols) of one vocabulary tile, the
+// first of them vocabulary entry n0.
+__device__ __forceinline__ VocabPart vocab_part(const Problem& p, const float (&v)[128], int n0,
+                                                int cols, int64_t want) {
+  VocabPart part{-INFINITY, 0.f, INT32_MAX, 0.f};
+  if (cols <= 0) return part;
+#pragma unroll
+  for (int c = 0; c < 128; c += 16)
+    if (c < cols)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) part.most = fmaxf(part.most, c + j < cols ? v[c + j] : -INFINITY);
+  const float base = part.most == -INFINITY ? 0.f : part.most;
+  float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+  for (int c = 0; c < 128; c += 16)
+    if (c < cols)
+#pragma unroll
+      for (int j = 0; j < 16; j += 2) {
+        s0 += c + j < cols ? ex2((v[c + j] - base) * kLog2e) : 0.f;
+        s1 += c + j + 1 < cols ? ex2((v[c + j + 1] - base) * kLog2e) : 0.f;
+      }
+  part.sum = s0 + s1;
+  if (p.tokens != nullptr) {
+    const bool here = want >= n0 && want < n0 + cols;
+    if (__any_sync(kFullMask, here)) {
+      const int at = here ? static_cast<int>(want - n0) : -1;
+#pragma unroll
+      for (int j = 0; j < 128; ++j)
+        if (j == at) part.chosen = v[j];
+    }
+    return part;
+  }
+#pragma unroll
+  for (int j = 127; j >= 0; --j)
+    if (j < cols && v[j] == part.most) part.at = n0 + j;
+  if (__any_sync(kFullMask, part.sum != part.sum)) {  // a NaN counts as the largest: the first
+#pragma unroll
+    for (int j = 127; j >= 0; --j)
+      if (j < cols && v[j] != v[j]) {
+        part.most = v[j];
+        part.at = n0 + j;
+      }
+  }
+  return part;
+}
+
+template <typename T, Kind kKind, int kAct, bool kPair>
 __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant__ GemmParams g) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int aborted;
+  constexpr int kCtas = kPair ? 2 : 1;
   const Problem& p = g.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = kPair ? static_cast<int>(tc::cluster_rank()) : 0;
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* ring = smem + kStagingBytes;
 
   if (threadIdx.x == 0) {
+    tc::prefetch_tensormap(&g.map_x);
+    tc::prefetch_tensormap(&g.map_w);
+    if (kKind == kGated) tc::prefetch_tensormap(&g.map_up);
     for (int i = 0; i < g.stages; ++i) {
       tc::mbar_init(&full[i], 1);
       tc::mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(&acc_full[i], 1);
-      tc::mbar_init(&acc_empty[i], 4);
+      tc::mbar_init(&acc_empty[i], kEpilogueWarps * kCtas);
     }
     aborted = 0;
     tc::fence_mbar_init();
   }
-  if (warp == 5) tc::tmem_alloc(&tmem_slot, 512);
+  if (warp == kEpilogueWarps + 1) {
+    if (kPair)
+      tc::tmem_alloc_pair(&tmem_slot, 512);
+    else
+      tc::tmem_alloc(&tmem_slot, 512);
+  }
   tc::tc_fence_before();
-  __syncthreads();
+  if (kPair)
+    tc::cluster_sync();
+  else
+    __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = tmem_slot;
 
   const int kblocks = (p.inner + kBlockK - 1) / kBlockK;
   const int tiles = g.row_tiles * g.col_tiles;
+  const int first = blockIdx.x / kCtas, step = gridDim.x / kCtas;
+  const int per_acc = kKind == kVocab ? kVocabBlocks : kblocks;  // blocks per accumulator
   bool ok = true;
 
-  if (warp == 4) {
-    if (lane == 0) {
-      const uint32_t bytes = g.box_m * 128 + g.load_n * 128 * (kKind == kGated ? 2 : 1);
-      uint32_t it = 0;
-      for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
-        const int m0 = tile % g.row_tiles * kTileM;
-        const int n0 = tile / g.row_tiles * g.set_n;
-        for (int kb = 0; kb < kblocks; ++kb, ++it) {
-          const int s = it % g.stages;
-          if (it >= static_cast<uint32_t>(g.stages) &&
-              !tc::mbar_wait(&empty[s], (it / g.stages - 1) & 1, kWaitLimit)) {
+  if (warp >= kEpilogueWarps) {
+    if constexpr (kKind == kVocab) tc::setmaxnreg_dec<kOtherRegs>();
+    if (warp == kEpilogueWarps) {
+      const bool both = kKind == kGated && !kPair;  // this CTA copies gate and up rows
+      const uint32_t bytes = (g.box_m + g.load_n * (both ? 2 : 1)) * 128 * kCtas;
+      const int shift = kPair && kKind != kGated ? rank * g.load_n : 0;
+      const CUtensorMap* map_b = kPair && kKind == kGated && rank == 1 ? &g.map_up : &g.map_w;
+      auto load = [&](uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {
+        if (kPair)
+          tc::tma_load_2d_pair(dst, map, bar, c0, c1);
+        else
+          tc::tma_load_2d(dst, map, bar, c0, c1);
+      };
+      Ring at;
+      for (int tile = first; ok && tile < tiles; tile += step) {
+        const int m0 = (tile % g.row_tiles * kCtas + rank) * kTileM;
+        const int n0 = tile / g.row_tiles * g.set_n + shift;
+        for (int k0 = 0; k0 < p.inner; k0 += kBlockK, at.next(g.stages)) {
+          // a fresh barrier's earlier phase counts as complete
+          if (!__all_sync(kFullMask, tc::mbar_wait(&empty[at.slot], at.parity ^ 1, kWaitLimit))) {
             ok = false;
             break;
           }
-          uint8_t* a = smem + s * g.stage_bytes;
-          uint8_t* b = a + kBytesA;
-          tc::mbar_expect_tx(&full[s], bytes);
-          tc::tma_load_2d(a, &g.map_x, &full[s], kb * kBlockK, m0);
-          for (int half = 0; half < (kKind == kGated ? 2 : 1); ++half) {
-            const CUtensorMap* map = half ? &g.map_up : &g.map_w;
-            uint8_t* dst = b + half * g.load_n * 128;
+          if (tc::elect_one()) {
+            uint64_t* bar = &full[at.slot];
+            uint8_t* a = ring + at.slot * g.stage_bytes;
+            uint8_t* b = a + g.box_m * 128;
+            // the pair's copies all complete on the first CTA's barrier
+            if (rank == 0) tc::mbar_expect_tx(bar, bytes);
+            load(a, &g.map_x, bar, k0, m0);
             if (g.w_mn) {
-              for (int n = 0; n < g.load_n; n += 64)
-                tc::tma_load_2d(dst + n * 128, map, &full[s], n0 + n, kb * kBlockK);
+              for (int n = 0; n < g.load_n; n += 64) load(b + n * 128, map_b, bar, n0 + n, k0);
+              if (both)
+                for (int n = 0; n < g.load_n; n += 64)
+                  load(b + (g.load_n + n) * 128, &g.map_up, bar, n0 + n, k0);
             } else {
-              tc::tma_load_2d(dst, map, &full[s], kb * kBlockK, n0);
+              load(b, map_b, bar, k0, n0);
+              if (both) load(b + g.load_n * 128, &g.map_up, bar, k0, n0);
             }
           }
+          __syncwarp();
         }
       }
     }
-  } else if (warp == 5) {
-    if (lane == 0) {
-      const uint32_t idesc = tc::idesc_f16(Fmt<T>::value, kTileM, g.tile_n, g.w_mn);
-      const uint32_t kstep_b = g.w_mn ? 2048 : 32;
-      const uint32_t lbo_b = g.w_mn ? 8192 : 16;
-      uint32_t it = 0, n = 0;
-      for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++n) {
-        const uint32_t buf = n & 1;
-        if (n >= 2 && !tc::mbar_wait(&acc_empty[buf], (n / 2 - 1) & 1, kWaitLimit)) {
-          ok = false;
-          break;
-        }
-        tc::tc_fence_after();
-        for (int kb = 0; kb < kblocks; ++kb, ++it) {
-          const int s = it % g.stages;
-          if (!tc::mbar_wait(&full[s], (it / g.stages) & 1, kWaitLimit)) {
+    if (warp == kEpilogueWarps + 1 && rank == 0) {
+      const uint32_t idesc = tc::idesc_f16(Fmt<T>::value, kTileM * kCtas, g.tile_n, g.w_mn);
+      const uint32_t kstep_b = (g.w_mn ? 2048 : 32) >> 4;  // in the descriptors' 16-byte units
+      const uint64_t a_desc = tc::smem_desc_sw128(tc::smem_u32(ring), 16, 1024);
+      const uint64_t b_desc =
+          tc::smem_desc_sw128(tc::smem_u32(ring) + g.box_m * 128, g.w_mn ? 8192 : 16, 1024);
+      const uint32_t a_hi = static_cast<uint32_t>(a_desc >> 32);
+      const uint32_t b_hi = static_cast<uint32_t>(b_desc >> 32);
+      const uint32_t stage_units = g.stage_bytes >> 4;
+      Ring at, acc;
+      for (int tile = first; ok && tile < tiles; tile += step) {
+        for (int kb = 0; ok && kb < kblocks; acc.next(2)) {
+          if (!__all_sync(kFullMask,
+                          tc::mbar_poll(&acc_empty[acc.slot], acc.parity ^ 1, kWaitLimit))) {
             ok = false;
             break;
           }
           tc::tc_fence_after();
-          const uint32_t a = tc::smem_u32(smem + s * g.stage_bytes);
-          const uint32_t b = a + kBytesA;
+          const uint32_t d = tmem + acc.slot * 256;
+          const int kb_end = min(kb + per_acc, kblocks);
+          for (uint32_t more = 0; kb < kb_end; ++kb, at.next(g.stages)) {
+            if (!__all_sync(kFullMask, tc::mbar_poll(&full[at.slot], at.parity, kWaitLimit))) {
+              ok = false;
+              break;
+            }
+            tc::tc_fence_after();
+            if (tc::elect_one()) {
+              const uint32_t a_lo = static_cast<uint32_t>(a_desc) + at.slot * stage_units;
+              const uint32_t b_lo = static_cast<uint32_t>(b_desc) + at.slot * stage_units;
 #pragma unroll
-          for (int ks = 0; ks < kBlockK / 16; ++ks)
-            tc::mma_f16_ss(tmem + buf * 256, tc::smem_desc_sw128(a + ks * 32, 16, 1024),
-                           tc::smem_desc_sw128(b + ks * kstep_b, lbo_b, 1024), idesc,
-                           kb > 0 || ks > 0);
-          tc::mma_commit(&empty[s]);
+              for (int ks = 0; ks < kBlockK / 16; ++ks) {
+                const uint64_t ad = tc::desc64(a_lo + ks * 2, a_hi);
+                const uint64_t bd = tc::desc64(b_lo + ks * kstep_b, b_hi);
+                if (kPair)
+                  tc::mma_f16_ss_pair(d, ad, bd, idesc, ks > 0 ? 1 : more);
+                else
+                  tc::mma_f16_ss(d, ad, bd, idesc, ks > 0 ? 1 : more);
+              }
+              if (kPair)
+                tc::mma_commit_pair(&empty[at.slot]);
+              else
+                tc::mma_commit(&empty[at.slot]);
+              if (kb == kb_end - 1) {
+                if (kPair)
+                  tc::mma_commit_pair(&acc_full[acc.slot]);
+                else
+                  tc::mma_commit(&acc_full[acc.slot]);
+              }
+            }
+            more = 1;
+            __syncwarp();
+          }
         }
-        if (ok) tc::mma_commit(&acc_full[buf]);
       }
     }
   } else {
+    if constexpr (kKind == kVocab) tc::setmaxnreg_inc<kSumRegs>();
+    uint8_t* staging = smem + warp * 4096;
+    const int half = warp >> 2;  // this thread's columns
+    const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
     uint32_t n = 0;
-    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
-      const uint32_t buf = n & 1;
-      ok = __all_sync(kFullMask, tc::mbar_wait(&acc_full[buf], (n / 2) & 1, kWaitLimit));
-      if (!ok) break;
+    auto wait_acc = [&]() {
+      ok = __all_sync(kFullMask, tc::mbar_wait(&acc_full[n & 1], (n / 2) & 1, kWaitLimit));
       tc::tc_fence_after();
-      const int col_tile = tile / g.row_tiles;
-      const int row = tile % g.row_tiles * kTileM + threadIdx.x;
-      const int n0 = col_tile * g.set_n;
-      const uint32_t taddr = tmem + buf * 256 + (static_cast<uint32_t>(warp) << 21);
-      if constexpr (kKind == kVocab) {
-        vocab_tile_part(g, taddr, row, n0, col_tile);
-      } else {
-        const int cols = min(g.set_n, p.outer - n0);
-        for (int c = 0; c < cols; c += 32) {
-          uint32_t v[32], up[32];
-          __syncwarp();
-          tc::tmem_ld32(taddr + c, v);
-          if constexpr (kKind == kGated) tc::tmem_ld32(taddr + g.set_n + c, up);
-          tc::tmem_ld_wait(v);
-          if constexpr (kKind == kGated) tc::tmem_ld_wait(up);
-          finish32<T, kKind, kAct>(p, g.vec, row, n0 + c, n0 + cols, v, up);
-        }
-      }
+      return ok;
+    };
+    auto release_acc = [&]() {
       tc::tc_fence_before();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&acc_empty[buf]);
+      if (lane == 0) {
+        if (kPair)
+          tc::mbar_arrive_at(&acc_empty[n & 1], 0);
+        else
+          tc::mbar_arrive(&acc_empty[n & 1]);
+      }
+      ++n;
+    };
+    for (int tile = first; ok && tile < tiles; tile += step) {
+      const int col_tile = tile / g.row_tiles;
+      const int row0 = (tile % g.row_tiles * kCtas + rank) * kTileM + (warp & 3) * 32;
+      const int n0 = col_tile * g.set_n;
+      if constexpr (kKind == kVocab) {
+        const int mine = g.tile_n / 2;  // a multiple of 16, at most 128
+        float v[128];
+        for (int kb = 0; kb < kblocks; kb += kVocabBlocks) {
+          if (!wait_acc()) break;
+          const uint32_t taddr = tmem + (n & 1) * 256 + lanes + half * mine;
+#pragma unroll
+          for (int c = 0; c < 128; c += 16) {
+            if (c < mine) {
+              uint32_t t[16];
+              tc::tmem_ld16(taddr + c, t);
+              tc::tmem_ld_wait(t);
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                v[c + j] = kb == 0 ? __uint_as_float(t[j]) : v[c + j] + __uint_as_float(t[j]);
+            }
+          }
+          release_acc();
+        }
+        if (!ok) break;
+        const int row = row0 + lane, at = n0 + half * mine;
+        const int64_t want = p.tokens != nullptr && row < p.rows ? p.tokens[row] : -1;
+        const VocabPart part = vocab_part(p, v, at, min(mine, p.outer - at), want);
+        if (row < p.rows)
+          *reinterpret_cast<float4*>(
+              &p.parts[static_cast<int64_t>(row) * p.tiles + col_tile * 2 + half]) =
+              make_float4(part.most, part.sum, __int_as_float(part.at), part.chosen);
+      } else {
+        if (!wait_acc()) break;
+        const uint32_t taddr = tmem + (n & 1) * 256 + lanes;
+        const int end = min(p.outer, n0 + g.set_n);
+        if (row0 < p.rows) {
+          for (int c = half * 32; c < end - n0; c += 64) {
+            uint32_t t[32];
+            float v[32];
+            __syncwarp();
+            tc::tmem_ld32(taddr + c, t);
+            if constexpr (kKind == kGated) {
+              uint32_t up[32];
+              tc::tmem_ld32(taddr + g.set_n + c, up);
+              tc::tmem_ld_wait(t);
+              tc::tmem_ld_wait(up);
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                v[j] = activate<false, kAct>(__uint_as_float(t[j])) * __uint_as_float(up[j]);
+              finish32<T, RLT_ACT_NONE>(p, g.vec, staging, row0, n0 + c, end, v);
+            } else {
+              tc::tmem_ld_wait(t);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(t[j]);
+              finish32<T, kAct>(p, g.vec, staging, row0, n0 + c, end, v);
+            }
+          }
+        }
+        release_acc();
+      }
     }
   }
   if (!ok) {  // a wait ran out: let copies in flight land before the memory goes
@@ -320,16 +466,23 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
   }
   __syncwarp();
   tc::tc_fence_before();
-  __syncthreads();
+  if (kPair)
+    tc::cluster_sync();
+  else
+    __syncthreads();
   if (aborted && threadIdx.x == 0) raise_status(p.status, kStatusTimeout);
-  if (warp == 5) {
+  if (warp == kEpilogueWarps + 1) {
     tc::tc_fence_after();
-    tc::tmem_dealloc(tmem, 512);
+    if (kPair)
+      tc::tmem_dealloc_pair(tmem, 512);
+    else
+      tc::tmem_dealloc(tmem, 512);
   }
 }
 
 // ---- few rows -----------------------------------------------------------------
 
+constexpr int kStreamThreads = 192;
 constexpr int kStreamRows = 64;     // activation rows that stream_kernel takes
 constexpr int kStreamStages = 12;
 constexpr int kStreamFeatures = 128;
@@ -347,7 +500,7 @@ struct StreamParams {
 };
 
 template <typename T, Kind kKind, int kAct>
-__global__ void __launch_bounds__(kThreads) stream_kernel(const __grid_constant__ StreamParams g) {
+__global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_constant__ StreamParams g) {
   constexpr int kOps = kKind == kGated ? 2 : 1;
   constexpr int kBytesW = kStreamFeatures * kBlockK * 2;
   extern __shared__ uint8_t smem_raw[];
@@ -385,53 +538,62 @@ __global__ void __launch_bounds__(kThreads) stream_kernel(const __grid_constant_
   bool ok = true;
 
   if (warp == 4) {
-    if (lane == 0) {
-      const uint32_t bytes = kOps * kBytesW + g.cols * 128;
-      for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {
-        const int s = it % g.stages;
-        if (it >= g.stages && !tc::mbar_wait(&empty[s], (it / g.stages - 1) & 1, kWaitLimit)) {
-          ok = false;
-          break;
-        }
-        uint8_t* w = smem + s * g.stage_bytes;
-        tc::mbar_expect_tx(&full[s], bytes);
+    const uint32_t bytes = kOps * kBytesW + g.cols * 128;
+    Ring at;
+    for (int kb = kb0; kb < kb1; ++kb, at.next(g.stages)) {
+      if (!__all_sync(kFullMask, tc::mbar_wait(&empty[at.slot], at.parity ^ 1, kWaitLimit))) {
+        ok = false;
+        break;
+      }
+      if (tc::elect_one()) {
+        uint64_t* bar = &full[at.slot];
+        uint8_t* w = smem + at.slot * g.stage_bytes;
+        tc::mbar_expect_tx(bar, bytes);
+#pragma unroll
         for (int op = 0; op < kOps; ++op) {
           const CUtensorMap* map = op ? &g.map_up : &g.map_w;
           uint8_t* dst = w + op * kBytesW;
           if (g.w_mn) {
-            tc::tma_load_2d(dst, map, &full[s], n0, kb * kBlockK);
-            tc::tma_load_2d(dst + 8192, map, &full[s], n0 + 64, kb * kBlockK);
+            tc::tma_load_2d(dst, map, bar, n0, kb * kBlockK);
+            tc::tma_load_2d(dst + 8192, map, bar, n0 + 64, kb * kBlockK);
           } else {
-            tc::tma_load_2d(dst, map, &full[s], kb * kBlockK, n0);
+            tc::tma_load_2d(dst, map, bar, kb * kBlockK, n0);
           }
         }
-        tc::tma_load_2d(w + kOps * kBytesW, &g.map_x, &full[s], kb * kBlockK, 0);
+        tc::tma_load_2d(w + kOps * kBytesW, &g.map_x, bar, kb * kBlockK, 0);
       }
+      __syncwarp();
     }
   } else if (warp == 5) {
-    if (lane == 0) {
-      const uint32_t idesc = tc::idesc_f16(Fmt<T>::value, kStreamFeatures, g.cols, 0, g.w_mn);
-      const uint32_t kstep_w = g.w_mn ? 2048 : 32;
-      const uint32_t lbo_w = g.w_mn ? 8192 : 16;
-      for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {
-        const int s = it % g.stages;
-        if (!tc::mbar_wait(&full[s], (it / g.stages) & 1, kWaitLimit)) {
-          ok = false;
-          break;
-        }
-        tc::tc_fence_after();
-        const uint32_t w = tc::smem_u32(smem + s * g.stage_bytes);
-        const uint32_t x = w + kOps * kBytesW;
+    const uint32_t idesc = tc::idesc_f16(Fmt<T>::value, kStreamFeatures, g.cols, 0, g.w_mn);
+    const uint32_t kstep_w = (g.w_mn ? 2048 : 32) >> 4;  // in 16-byte units
+    const uint64_t w_desc = tc::smem_desc_sw128(tc::smem_u32(smem), g.w_mn ? 8192 : 16, 1024);
+    const uint64_t x_desc = tc::smem_desc_sw128(tc::smem_u32(smem) + kOps * kBytesW, 16, 1024);
+    const uint32_t w_hi = static_cast<uint32_t>(w_desc >> 32);
+    const uint32_t x_hi = static_cast<uint32_t>(x_desc >> 32);
+    Ring at;
+    uint32_t more = 0;
+    for (int kb = kb0; kb < kb1; ++kb, at.next(g.stages)) {
+      if (!__all_sync(kFullMask, tc::mbar_poll(&full[at.slot], at.parity, kWaitLimit))) {
+        ok = false;
+        break;
+      }
+      tc::tc_fence_after();
+      if (tc::elect_one()) {
+        const uint32_t w_lo = static_cast<uint32_t>(w_desc) + at.slot * (g.stage_bytes >> 4);
+        const uint32_t x_lo = static_cast<uint32_t>(x_desc) + at.slot * (g.stage_bytes >> 4);
 #pragma unroll
         for (int ks = 0; ks < kBlockK / 16; ++ks)
 #pragma unroll
           for (int op = 0; op < kOps; ++op)
             tc::mma_f16_ss(tmem + op * kStreamRows,
-                           tc::smem_desc_sw128(w + op * kBytesW + ks * kstep_w, lbo_w, 1024),
-                           tc::smem_desc_sw128(x + ks * 32, 16, 1024), idesc, it > 0 || ks > 0);
-        tc::mma_commit(&empty[s]);
+                           tc::desc64(w_lo + op * (kBytesW >> 4) + ks * kstep_w, w_hi),
+                           tc::desc64(x_lo + ks * 2, x_hi), idesc, ks > 0 ? 1 : more);
+        tc::mma_commit(&empty[at.slot]);
+        if (kb == kb1 - 1) tc::mma_commit(&acc_full);
       }
-      if (ok) tc::mma_commit(&acc_full);
+      more = 1;
+      __syncwarp();
     }
   }
   __syncwarp();
@@ -483,7 +645,7 @@ __global__ void __launch_bounds__(kThreads) stream_kernel(const __grid_constant_
       for (int e = 0; e < 4; ++e)
         if (n + e < p.outer) b[e] = to_f32<T>(static_cast<const T*>(p.bias)[n + e]);
 #pragma unroll 2
-    for (int row = rank + warp * g.splits; row < p.rows; row += kThreads / 32 * g.splits) {
+    for (int row = rank + warp * g.splits; row < p.rows; row += kStreamThreads / 32 * g.splits) {
       float r[4] = {0.f, 0.f, 0.f, 0.f};
       if (kKind == kLinear && res != nullptr)
 #pragma unroll
@@ -569,42 +731,87 @@ bool encode2d(CUtensorMap* map, int32_t dtype, const void* base, int line, int l
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Dynamic shared memory of kKernel raised once per device.
+// Dynamic shared memory of kKernel raised (and its register count checked) once
+// per device.
 template <auto kKernel>
-cudaError_t allow_smem(int bytes) {
+cudaError_t allow_smem(int bytes, int least_regs = 0) {
   static std::atomic<bool> done[64];
   int dev = 0;
   if (const cudaError_t e = cudaGetDevice(&dev)) return e;
   if (dev >= 0 && dev < 64 && done[dev].load()) return cudaSuccess;
-  const cudaError_t e =
-      cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  cudaError_t e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && least_regs > 0) {
+    // with fewer registers at launch a warpgroup's increase could never be granted
+    cudaFuncAttributes attr{};
+    e = cudaFuncGetAttributes(&attr, kKernel);
+    if (e == cudaSuccess && attr.numRegs < least_regs) e = cudaErrorInvalidConfiguration;
+  }
   if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev].store(true);
   return e;
 }
 
 template <typename T, Kind kKind, int kAct>
 int launch(const GemmParams& g, int ctas, cudaStream_t stream) {
-  constexpr auto kernel = gemm_kernel<T, kKind, kAct>;
-  if (const cudaError_t e = allow_smem<kernel>(kSmemBudget + 1024)) return static_cast<int>(e);
-  kernel<<<ctas, kThreads, g.stages * g.stage_bytes + 1024, stream>>>(g);
-  return launch_status(cudaGetLastError());
+  const int regs = kKind == kVocab ? kLaunchRegs : 0;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kStagingBytes + g.ring_bytes + 1024;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = g.pair ? 2 : 1;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (g.pair) {
+    constexpr auto kernel = gemm_kernel<T, kKind, kAct, true>;
+    if (const cudaError_t e = allow_smem<kernel>(kSmemBudget, regs)) return static_cast<int>(e);
+    return launch_status(cudaLaunchKernelEx(&cfg, kernel, g));
+  }
+  constexpr auto kernel = gemm_kernel<T, kKind, kAct, false>;
+  if (const cudaError_t e = allow_smem<kernel>(kSmemBudget, regs)) return static_cast<int>(e);
+  return launch_status(cudaLaunchKernelEx(&cfg, kernel, g));
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
 
-// Output features per tile: the width whose tiles waste least of the last
-// wave of CTAs, the widest among equals. `step`: what the weights' layout asks.
-int choose_set(int outer, int row_tiles, int widest, int step, int ctas) {
-  int best = widest;
+// How gemm_kernel tiles a problem: output features per tile, and whether a
+// tile is a pair of CTAs' (256 rows) or one CTA's (128).
+struct Tiling {
+  int set_n;
+  bool pair;
+};
+
+// The tiling that a model of a tile's cycles says is fastest. Per 64 input
+// features a tile of N columns takes 2 N cycles of arithmetic, and its copies
+// arrive at about 60 bytes a cycle from L2, or 35 where all SMs stream weights
+// that are read once (one row tile). Tiles run in waves; each pays a start, and
+// the last wave's epilogue is exposed.
+Tiling choose_tiling(Kind kind, const Problem& p, int ctas) {
+  const int per = kind == kGated ? 2 : 1;
+  const bool mn = p.w_ks != 1;
+  const double kblocks = ceil_div(p.inner, kBlockK);
+  Tiling best{256 / per, false};
   double least = 1e300;
-  for (int n = widest; n >= step; n -= step) {
-    const int64_t tiles = static_cast<int64_t>(ceil_div(outer, n)) * row_tiles;
-    const int64_t waves = (tiles + ctas - 1) / ctas;
-    // a tile's time: its columns plus what every tile pays
-    const double cost = static_cast<double>(waves) * (n + 32);
-    if (cost < least * 0.999) {
-      least = cost;
-      best = n;
+  for (int pair = p.rows > kTileM ? 1 : 0; pair >= 0; --pair) {
+    const int64_t row_tiles = ceil_div(p.rows, pair ? 2 * kTileM : kTileM);
+    // a pair's CTAs copy half of B each: whole 64-feature blocks MN-major
+    const int finest = mn ? (pair && per == 1 ? 128 : 64) : 32 / per;
+    const int workers = pair ? ctas / 2 : ctas;
+    for (int set = 256 / per; set >= finest; set -= finest) {
+      const int n = set * per;
+      const int64_t tiles = row_tiles * ceil_div(p.outer, set);
+      const double waves = static_cast<double>((tiles + workers - 1) / workers);
+      const int box = p.rows < kTileM ? p.rows : kTileM;
+      const double rate = row_tiles == 1 && tiles > workers / 2 ? 35.0 : 60.0;
+      const double copies = (box + (pair ? n / 2 : n)) * 128 / rate;
+      const double cycles = copies > 2.0 * n ? copies : 2.0 * n;
+      const double cost = waves * (kblocks * cycles + 600) + 12 * n;
+      if (cost < least * 0.999) {
+        least = cost;
+        best = Tiling{set, pair == 1};
+      }
     }
   }
   return best;
@@ -613,10 +820,10 @@ int choose_set(int outer, int row_tiles, int widest, int step, int ctas) {
 template <typename T, Kind kKind, int kAct>
 int launch(const StreamParams& g, int tiles, cudaStream_t stream) {
   constexpr auto kernel = stream_kernel<T, kKind, kAct>;
-  if (const cudaError_t e = allow_smem<kernel>(kSmemBudget + 1024)) return static_cast<int>(e);
+  if (const cudaError_t e = allow_smem<kernel>(kSmemBudget)) return static_cast<int>(e);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(tiles * g.splits));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(kStreamThreads);
   cfg.dynamicSmemBytes = g.stages * g.stage_bytes + 1024;
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
@@ -631,14 +838,17 @@ int launch(const StreamParams& g, int tiles, cudaStream_t stream) {
 // The kernel for a launch's type and activation.
 template <Kind kKind, typename T, typename Params>
 int by_activation(const Params& g, int ctas, cudaStream_t stream) {
-  if constexpr (kKind == kVocab) return launch<T, kKind, RLT_ACT_NONE>(g, ctas, stream);
-  switch (g.p.act) {
-    case RLT_ACT_SILU: return launch<T, kKind, RLT_ACT_SILU>(g, ctas, stream);
-    case RLT_ACT_GELU: return launch<T, kKind, RLT_ACT_GELU>(g, ctas, stream);
-    case RLT_ACT_GELU_TANH: return launch<T, kKind, RLT_ACT_GELU_TANH>(g, ctas, stream);
-    case RLT_ACT_RELU: return launch<T, kKind, RLT_ACT_RELU>(g, ctas, stream);
-    case RLT_ACT_SIGMOID: return launch<T, kKind, RLT_ACT_SIGMOID>(g, ctas, stream);
-    default: return launch<T, kKind, RLT_ACT_NONE>(g, ctas, stream);
+  if constexpr (kKind == kVocab) {
+    return launch<T, kKind, RLT_ACT_NONE>(g, ctas, stream);
+  } else {
+    switch (g.p.act) {
+      case RLT_ACT_SILU: return launch<T, kKind, RLT_ACT_SILU>(g, ctas, stream);
+      case RLT_ACT_GELU: return launch<T, kKind, RLT_ACT_GELU>(g, ctas, stream);
+      case RLT_ACT_GELU_TANH: return launch<T, kKind, RLT_ACT_GELU_TANH>(g, ctas, stream);
+      case RLT_ACT_RELU: return launch<T, kKind, RLT_ACT_RELU>(g, ctas, stream);
+      case RLT_ACT_SIGMOID: return launch<T, kKind, RLT_ACT_SIGMOID>(g, ctas, stream);
+      default: return launch<T, kKind, RLT_ACT_NONE>(g, ctas, stream);
+    }
   }
 }
 template <Kind kKind, typename Params>
@@ -653,7 +863,7 @@ int run_stream(Kind kind, const Problem& p, int32_t dtype, int ctas, cudaStream_
   g.p = p;
   g.w_mn = p.w_ks != 1;
   g.cols = ceil_div(p.rows, 16) * 16;
-  g.vec = p.outer % 4 == 0 && p.o_rs % 4 == 0 && reinterpret_cast<uintptr_t>(p.out) % 8 == 0;
+  g.vec = p.outer % 4 == 0 && p.o_rs % 4 == 0 && aligned8(p.out);
   g.stage_bytes = ops * kStreamFeatures * kBlockK * 2 + g.cols * 128;
   const int tiles = ceil_div(p.outer, kStreamFeatures);
   const int kblocks = ceil_div(p.inner, kBlockK);
@@ -682,28 +892,31 @@ int run_stream(Kind kind, const Problem& p, int32_t dtype, int ctas, cudaStream_
 
 }  // namespace
 
-int tc_vocab_tile(const Problem& p, int ctas) {
-  const bool mn = p.w_ks != 1;
-  return choose_set(p.outer, ceil_div(p.rows, kTileM), 256, mn ? 64 : 16, ctas);
+int tc_vocab_parts(const Problem& p, int ctas) {
+  return 2 * ceil_div(p.outer, choose_tiling(kVocab, p, ctas).set_n);
 }
 
 int run_tc(Kind kind, const Problem& p, int32_t dtype, int ctas, cudaStream_t stream) {
   if (kind != kVocab && p.rows <= kStreamRows) return run_stream(kind, p, dtype, ctas, stream);
   GemmParams g{};
   g.p = p;
+  const Tiling tiling = choose_tiling(kind, p, ctas);
+  g.pair = tiling.pair;
+  g.set_n = tiling.set_n;
   g.w_mn = p.w_ks != 1;
-  g.row_tiles = ceil_div(p.rows, kTileM);
+  g.row_tiles = ceil_div(p.rows, g.pair ? 2 * kTileM : kTileM);
   g.box_m = p.rows >= kTileM ? kTileM : ceil_div(p.rows, 8) * 8;
-  g.set_n = kind == kVocab ? tc_vocab_tile(p, ctas)
-                           : choose_set(p.outer, g.row_tiles, kind == kGated ? 128 : 256,
-                                        g.w_mn ? 64 : 16, ctas);
-  g.load_n = g.set_n;
   g.tile_n = kind == kGated ? 2 * g.set_n : g.set_n;
+  g.load_n = g.pair ? g.tile_n / 2 : g.set_n;
   g.col_tiles = ceil_div(p.outer, g.set_n);
-  g.stage_bytes = kBytesA + g.tile_n * 128;
-  g.stages = kSmemBudget / g.stage_bytes < kMaxStages ? kSmemBudget / g.stage_bytes : kMaxStages;
-  g.vec = aligned16(p.out) && p.o_rs % 8 == 0 && (p.bias == nullptr || aligned16(p.bias)) &&
-          (p.residual == nullptr || (aligned16(p.residual) && p.r_rs % 8 == 0));
+  g.stage_bytes = (g.box_m + (g.pair ? g.load_n : g.tile_n)) * 128;
+  // the tensor core reads 128 rows of A whatever was copied: past the last
+  // stage's end that is still inside the ring
+  g.stages = (kSmemBudget - kStagingBytes - 1024 - (kTileM - g.box_m) * 128) / g.stage_bytes;
+  if (g.stages > kMaxStages) g.stages = kMaxStages;
+  g.ring_bytes = g.stages * g.stage_bytes + (kTileM - g.box_m) * 128;
+  g.vec = aligned8(p.out) && p.o_rs % 4 == 0 && aligned8(p.bias) && aligned8(p.residual) &&
+          p.r_rs % 4 == 0;
   if (static_cast<int64_t>(g.row_tiles) * g.col_tiles > INT32_MAX) return RLT_E_SHAPE;
   bool ok = encode2d(&g.map_x, dtype, p.x, p.inner, p.rows, p.x_rs, g.box_m);
   for (int half = 0; half < (kind == kGated ? 2 : 1); ++half) {
@@ -714,7 +927,8 @@ int run_tc(Kind kind, const Problem& p, int32_t dtype, int ctas, cudaStream_t st
   }
   if (!ok) return RLT_E_DEVICE;
   const int tiles = g.row_tiles * g.col_tiles;
-  if (tiles < ctas) ctas = tiles;
+  if (g.pair) ctas = ctas / 2 < tiles ? ctas / 2 * 2 : tiles * 2;
+  if (tiles < ctas) ctas = g.pair ? ctas : tiles;
   switch (kind) {
     case kLinear: return by_type<kLinear>(g, dtype, ctas, stream);
     case kGated: return by_type<kGated>(g, dtype, ctas, stream);

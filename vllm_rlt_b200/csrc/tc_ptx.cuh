@@ -102,6 +102,20 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, long l
   return true;
 }
 
+// One lane of a converged warp. The compiler knows the branch it guards to be
+// one thread's, so the TMA and tensor-core instructions in it take their
+// operands from uniform registers directly (behind a test of the lane number
+// each is wrapped in a loop over the lanes).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
 // ---- TMA (tiled, no multicast) ------------------------------------------
 
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar,
