@@ -89,7 +89,7 @@ def test_head_arguments():
 def test_weight_layouts():
     def strides(w):
         w = FakeCuda(w)
-        return projections._operands(fake(2, w.shape[1], dtype=w.dtype), w, "")[4:6]
+        return projections._operands(fake(2, w.shape[1], dtype=w.dtype), w, "")[5:7]
 
     assert strides(torch.zeros(4, 8)) == (8, 1)
     assert strides(torch.zeros(8, 4).t()) == (1, 4)

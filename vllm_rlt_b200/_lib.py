@@ -170,6 +170,19 @@ def status_word(device: torch.device) -> torch.Tensor:
     return word
 
 
+_status_ptrs: dict[int, int] = {}
+
+
+def status_ptr(device: torch.device) -> int:
+    """Address of ``status_word(device)``, which lives as long as the process."""
+    address = _status_ptrs.get(device.index)
+    if address is None:
+        address = status_word(device).data_ptr()
+        if device.index is not None:
+            _status_ptrs[device.index] = address
+    return address
+
+
 def read_status(device: torch.device, reset: bool = True) -> list[str]:
     """Synchronise and return (and by default clear) the raised error bits."""
     word = status_word(device)

@@ -159,20 +159,20 @@ __device__ __forceinline__ void finish32(const Problem& p, int vec, uint8_t* sta
     if (n + lane < end) {
       const int at = n + lane;
       const float b = bias != nullptr ? to_f32<T>(bias[at]) : 0.f;
-      for (int row = 0; row < rows; row += 8) {
-        float y[8];
+      for (int row = 0; row < rows; row += 16) {
+        float y[16];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < 16; ++i)
           y[i] = res != nullptr && row + i < rows ? to_f32<T>(res[(row0 + row + i) * p.r_rs + at])
                                                   : 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 16; ++i) {
           const float f = *reinterpret_cast<const float*>(
-              staging + (row + i) * 128 + (((lane >> 2) ^ i) << 4) + (lane & 3) * 4);
+              staging + (row + i) * 128 + (((lane >> 2) ^ (i & 7)) << 4) + (lane & 3) * 4);
           y[i] += activate<false, kAct>(f + b);
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < 16; ++i)
           if (row + i < rows) out[(row0 + row + i) * p.o_rs + at] = from_f32<T>(y[i]);
       }
     }
@@ -807,7 +807,8 @@ Tiling choose_tiling(Kind kind, const Problem& p, int ctas) {
       const double rate = row_tiles == 1 && tiles > workers / 2 ? 35.0 : 60.0;
       const double copies = (box + (pair ? n / 2 : n)) * 128 / rate;
       const double cycles = copies > 2.0 * n ? copies : 2.0 * n;
-      const double cost = waves * (kblocks * cycles + 600) + 12 * n;
+      // a warp finishes every other chunk of 32 columns
+      const double cost = waves * (kblocks * cycles + 600) + ceil_div(n, 64) * 1500;
       if (cost < least * 0.999) {
         least = cost;
         best = Tiling{set, pair == 1};

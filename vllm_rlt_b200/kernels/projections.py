@@ -26,13 +26,10 @@ ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2, "gelu_tanh": 3, "relu": 4, "sigmoi
 
 def _operands(x, weight, what):
     """Check x [rows, in] and weight [out, in]; returns x with contiguous rows,
-    rows, in, out, the weight's strides (one of them 1) and the dtype's code."""
-    try:
-        rows, inner = x.shape
-        outer, inner_w = weight.shape
-    except ValueError:
-        inner, inner_w = 0, -1
-    if inner != inner_w:
+    rows, in, out, x's row stride, the weight's strides (one of them 1), the
+    dtype's code and the device."""
+    shape, wshape = x.shape, weight.shape
+    if len(shape) != 2 or len(wshape) != 2 or shape[1] != wshape[1]:
         raise ValueError(f"{what}: expected x [rows, in] and weight [out, in]")
     device, dtype = x.device, x.dtype
     if device.type != "cuda":
@@ -42,32 +39,37 @@ def _operands(x, weight, what):
         raise ValueError(f"{what}: x and weight must share a float32, float16 or bfloat16 dtype")
     if weight.device != device:
         raise ValueError(f"{what}: all tensors must live on the same device")
+    rows, inner = shape
     if inner == 0:
         raise ValueError(f"{what}: in_features must be positive")
     ns, ks = weight.stride()
     if ks == 1 or inner == 1:
         ks = 1
-    elif ns == 1 or outer == 1:
+    elif ns == 1 or wshape[0] == 1:
         ns = 1
     else:
         raise ValueError(f"{what}: one dimension of weight must be contiguous")
-    if x.stride(1) != 1:
-        x = x.contiguous()
-    return x, rows, inner, outer, ns, ks, code
+    xs, unit = x.stride()
+    if unit != 1:
+        x, xs = x.contiguous(), inner
+    return x, rows, inner, wshape[0], xs, ns, ks, code, device
 
 
-def _rows_like(t, x, outer, name, what):
-    if t.shape != (x.shape[0], outer) or t.dtype != x.dtype or t.device != x.device:
+def _rows_like(t, rows, outer, x, name, what):
+    if t.shape != (rows, outer) or t.dtype != x.dtype or t.device != x.device:
         raise ValueError(f"{what}: {name} must be [rows, out] of x's dtype and device")
 
 
 def _output(out, x, rows, outer, what):
+    """The result tensor and its row stride."""
     if out is None:
-        return x.new_empty((rows, outer))
-    _rows_like(out, x, outer, "out", what)
-    if outer > 1 and out.stride(1) != 1 or rows > 1 and out.stride(0) < outer:
+        return torch.empty_strided((rows, outer), (outer, 1), dtype=x.dtype,
+                                   device=x.device), outer
+    _rows_like(out, rows, outer, x, "out", what)
+    stride, unit = out.stride()
+    if outer > 1 and unit != 1 or rows > 1 and stride < outer:
         raise ValueError(f"{what}: rows of out must be contiguous and apart")
-    return out
+    return out, stride
 
 
 def _activation(name, what):
@@ -77,20 +79,19 @@ def _activation(name, what):
         raise ValueError(f"{what}: activation must be one of {list(ACTIVATIONS)}") from None
 
 
-def _run(device, what, entry, need, *args):
-    """Call ``entry(workspace, bytes, status, stream)`` on ``device``; scratch
-    is only asked for, and allocated, by the few calls whose operands have to be
-    copied into aligned rows (they are refused without it)."""
-    index = device.index
-    if index != torch.cuda.current_device():
+def _run(device, what, entry, head, tail, need, operands):
+    """``entry(*head, workspace, bytes, status, *tail, stream)`` on ``device``.
+    Scratch is asked for, and allocated, only by calls that are refused without:
+    the vocabulary head, and operands that have to be copied into aligned rows."""
+    if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
-            return _run(device, what, entry, need, *args)
-    status, stream = _lib.status_word(device).data_ptr(), _lib.stream_of(device)
-    rc = entry(None, 0, status, stream)
+            return _run(device, what, entry, head, tail, need, operands)
+    status, stream = _lib.status_ptr(device), _lib.stream_of(device)
+    rc = entry(*head, None, 0, status, *tail, stream)
     if rc == _lib.E_WORKSPACE:
-        size = need(*args)
+        size = need(*operands)
         scratch = torch.empty(size, dtype=torch.uint8, device=device)
-        rc = entry(scratch.data_ptr(), size, status, stream)
+        rc = entry(*head, scratch.data_ptr(), size, status, *tail, stream)
     if rc:
         _lib.check(rc, what)
 
@@ -103,30 +104,29 @@ def linear(x, weight, bias=None, *, activation=None, residual=None, out=None):
     "gelu_tanh", "relu" or "sigmoid". ``out`` may be ``residual`` itself and
     must not overlap any other argument."""
     what = "linear"
-    x, rows, inner, outer, ns, ks, code = _operands(x, weight, what)
+    x, rows, inner, outer, xs, ns, ks, code, device = _operands(x, weight, what)
     act = _activation(activation, what)
     bias_ptr = residual_ptr = None
-    residual_stride = 0
+    rs = 0
     if bias is not None:
-        if bias.shape != (outer,) or bias.dtype != x.dtype or bias.device != x.device:
+        if bias.shape != (outer,) or bias.dtype != x.dtype or bias.device != device:
             raise ValueError(f"{what}: bias must be [out] of x's dtype and device")
-        bias = bias.contiguous()
+        if bias.stride(0) != 1:
+            bias = bias.contiguous()
         bias_ptr = bias.data_ptr()
     if residual is not None:
-        _rows_like(residual, x, outer, "residual", what)
-        if residual.stride(1) != 1:
-            residual = residual.contiguous()
-        residual_ptr, residual_stride = residual.data_ptr(), residual.stride(0)
-    result = _output(out, x, rows, outer, what)
+        _rows_like(residual, rows, outer, x, "residual", what)
+        rs, unit = residual.stride()
+        if unit != 1:
+            residual, rs = residual.contiguous(), outer
+        residual_ptr = residual.data_ptr()
+    result, os = _output(out, x, rows, outer, what)
     if rows == 0 or outer == 0:
         return result
-    lib, xp, wp, xs = _lib.load(), x.data_ptr(), weight.data_ptr(), x.stride(0)
-    op, os = result.data_ptr(), result.stride(0)
-    _run(x.device, what,
-         lambda scratch, size, status, stream: lib.rlt_linear(
-             xp, wp, bias_ptr, residual_ptr, op, scratch, size, status, code, rows, inner, outer,
-             act, xs, ns, ks, residual_stride, os, stream),
-         lib.rlt_linear_workspace_bytes, xp, wp, code, rows, inner, outer, 0, xs, ns, ks)
+    lib, xp, wp = _lib.load(), x.data_ptr(), weight.data_ptr()
+    _run(device, what, lib.rlt_linear, (xp, wp, bias_ptr, residual_ptr, result.data_ptr()),
+         (code, rows, inner, outer, act, xs, ns, ks, rs, os),
+         lib.rlt_linear_workspace_bytes, (xp, wp, code, rows, inner, outer, 0, xs, ns, ks))
     return result
 
 
@@ -134,29 +134,25 @@ def gated_linear(x, weight, *, activation="silu", out=None):
     """``act(x @ gate.t()) * (x @ up.t())`` in one kernel, ``weight`` being
     ``[gate; up]``, ``[2 * features, in]``. Returns ``[rows, features]``."""
     what = "gated linear"
-    x, rows, inner, outer, ns, ks, code = _operands(x, weight, what)
+    x, rows, inner, outer, xs, ns, ks, code, device = _operands(x, weight, what)
     if outer % 2:
         raise ValueError(f"{what}: weight must hold as many gate rows as up rows")
     outer //= 2
     act = _activation(activation, what)
-    result = _output(out, x, rows, outer, what)
+    result, os = _output(out, x, rows, outer, what)
     if rows == 0 or outer == 0:
         return result
-    lib, xp, wp, xs = _lib.load(), x.data_ptr(), weight.data_ptr(), x.stride(0)
-    op, os = result.data_ptr(), result.stride(0)
-    _run(x.device, what,
-         lambda scratch, size, status, stream: lib.rlt_gated_linear(
-             xp, wp, op, scratch, size, status, code, rows, inner, outer, act, xs, ns, ks, os,
-             stream),
-         lib.rlt_linear_workspace_bytes, xp, wp, code, rows, inner, outer, 1, xs, ns, ks)
+    lib, xp, wp = _lib.load(), x.data_ptr(), weight.data_ptr()
+    _run(device, what, lib.rlt_gated_linear, (xp, wp, result.data_ptr()),
+         (code, rows, inner, outer, act, xs, ns, ks, os),
+         lib.rlt_linear_workspace_bytes, (xp, wp, code, rows, inner, outer, 1, xs, ns, ks))
     return result
 
 
 def _vocab_head(hidden, weight, tokens, what):
-    hidden, rows, inner, vocab, ns, ks, code = _operands(hidden, weight, what)
+    hidden, rows, inner, vocab, hs, ns, ks, code, device = _operands(hidden, weight, what)
     if vocab == 0:
         raise ValueError(f"{what}: the vocabulary must not be empty")
-    device = hidden.device
     chosen = chosen_ptr = tokens_ptr = None
     if tokens is None:
         chosen = torch.empty(rows, dtype=torch.int64, device=device)
@@ -166,13 +162,10 @@ def _vocab_head(hidden, weight, tokens, what):
     logprobs = torch.empty(rows, dtype=torch.float32, device=device)
     if rows == 0:
         return chosen, logprobs
-    lib, hp, wp, hs = _lib.load(), hidden.data_ptr(), weight.data_ptr(), hidden.stride(0)
-    lp = logprobs.data_ptr()
-    _run(device, what,
-         lambda scratch, size, status, stream: lib.rlt_vocab_head(
-             hp, wp, tokens_ptr, chosen_ptr, lp, scratch, size, status, code, rows, inner, vocab,
-             hs, ns, ks, stream),
-         lib.rlt_vocab_head_workspace_bytes, hp, wp, code, rows, inner, vocab, hs, ns, ks)
+    lib, hp, wp = _lib.load(), hidden.data_ptr(), weight.data_ptr()
+    _run(device, what, lib.rlt_vocab_head, (hp, wp, tokens_ptr, chosen_ptr, logprobs.data_ptr()),
+         (code, rows, inner, vocab, hs, ns, ks),
+         lib.rlt_vocab_head_workspace_bytes, (hp, wp, code, rows, inner, vocab, hs, ns, ks))
     return chosen, logprobs
 
 
