@@ -404,10 +404,10 @@ int rlt_silu_mul(const void* gate_up, void* out, int32_t dtype, int32_t rows,
 /* ---- projections ---- */
 
 /* Scratch of rlt_linear and rlt_gated_linear, in bytes: copies of x and of the
- * weights in rows of whole 16-byte units, for 16-bit operands that are not laid
- * out so (a pointer that is not 16-byte aligned, a stride that is not a
- * multiple of 8 elements or shorter than its row). 0 when none is needed, and
- * always for fp32. `gated`: 0 or 1; out_features counts one half then. */
+ * weights in rows of whole 16-byte units, for operands that are not laid out
+ * so (a pointer that is not 16-byte aligned, a stride that is not a multiple
+ * of 16 bytes or shorter than its row). 0 when none is needed. `gated`: 0 or 1;
+ * out_features counts one half then. */
 size_t rlt_linear_workspace_bytes(const void* x, const void* weight, int32_t dtype, int32_t rows,
                                   int32_t in_features, int32_t out_features, int32_t gated,
                                   int64_t x_row_stride, int64_t weight_out_stride,
@@ -422,7 +422,8 @@ size_t rlt_linear_workspace_bytes(const void* x, const void* weight, int32_t dty
  * tensor as residual and overlaps nothing else. in_features >= 1; rows or
  * out_features of 0 launch nothing. act: RLT_ACT_*. A row's result depends on
  * that row, the weights, and the launch shape only, and repeats bit for bit.
- * bf16 and fp16 run on the tensor cores, fp32 in fp32 multiply-adds.
+ * All types run on the tensor cores, fp32 as three bf16 parts per number (six
+ * products of parts, to about the error of fp32 multiply-adds).
  * Replaces the projections of vllm_rlt/models/ouro.py:96-123 with what follows
  * them, and the exit gate's product, bias and sigmoid (:209-217). */
 int rlt_linear(const void* x, const void* weight, const void* bias, const void* residual,

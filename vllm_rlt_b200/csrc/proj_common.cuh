@@ -105,10 +105,26 @@ __device__ __forceinline__ void fold(VocabPart& a, const VocabPart& b) {
   a.chosen += b.chosen;
 }
 
-// Tensor-core path (16-bit operands whose pointers and strides TMA accepts).
+// Launch attributes of these kernels: the cluster, and leave to start before
+// the stream's previous kernel has ended (they wait for it themselves).
+inline unsigned launch_attributes(cudaLaunchAttribute (&attrs)[2], int cluster) {
+  attrs[0] = {};
+  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[0].val.programmaticStreamSerializationAllowed = 1;
+  if (cluster == 1) return 1;
+  attrs[1] = {};
+  attrs[1].id = cudaLaunchAttributeClusterDimension;
+  attrs[1].val.clusterDim.x = cluster;
+  attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
+  return 2;
+}
+
+// 16-bit operands, and fp32 ones, whose pointers and strides TMA accepts.
 int run_tc(Kind kind, const Problem& p, int32_t dtype, int ctas, cudaStream_t stream);
-// Vocabulary records per row that it leaves.
+int run_split(Kind kind, const Problem& p, int ctas, cudaStream_t stream);
+// Vocabulary records per row that they leave.
 int tc_vocab_parts(const Problem& p, int ctas);
+int split_vocab_parts(const Problem& p);
 
 }  // namespace proj
 }  // namespace rlt

@@ -1,0 +1,459 @@
+// Projections of fp32 tensors on the tensor cores.
+//
+// An fp32 number is the sum of three bf16 numbers: its upper 8 significand bits
+// h, the next 8 m and the last 8 l, each split off by truncation, which is
+// exact. A product of two fp32 numbers is then the nine products of their
+// parts, each exact in fp32; the six of them down to 2^-16 of the largest are
+// formed (h h; h m, m h, m m, h l, l h) and what is left out is below 2^-23 of
+// the product, a rounding of fp32 arithmetic. bf16 products run 32 times as
+// fast as fp32 multiply-adds here, so six of them still are five times faster.
+//
+// The tensor core truncates as it accumulates, an error of one sign that grows
+// with the number of steps. h h and the five small products therefore have an
+// accumulator each (the small one's truncations are 2^-8 smaller), at most 512
+// input features go into them, and those sums are added in registers, rounded
+// to nearest.
+//
+// Infinities: a part of an infinity times a part that is zero would be NaN where
+// fp32 arithmetic gives an infinity. Any NaN that comes out is recomputed by
+// fp32 multiply-adds from the operands, so both end up as they would there.
+//
+// A CTA (18 warps) takes a tile of 128 rows by 128 weight rows over its share of
+// the input features; a cluster of up to 8 CTAs shares a tile when there are few.
+// Warp 16 copies slices of 32 input features (fp32, 128 bytes) by TMA, warps
+// 8-15 split them into parts in shared memory, warp 17 issues the products,
+// warps 0-7 gather the sums. Per slice of 128 x 128 shared memory moves 32 KB
+// in, 80 KB through the split and 96 KB into the tensor core, about 1660
+// cycles against 768 of arithmetic: that traffic bounds the kernel.
+#include "proj_tc.cuh"
+
+namespace rlt {
+namespace proj {
+namespace {
+
+constexpr int kSplitThreads = 18 * 32;
+constexpr int kSlice = 32;                   // input features per slice
+constexpr int kTile = 128;                   // rows, and weight rows, of a tile
+constexpr int kRawBytes = kTile * 128;       // one operand's slice as it arrives
+constexpr int kPartBytes = kTile * kSlice * 2;
+constexpr int kRawStages = 3, kPartStages = 2;
+constexpr int kRawStage = 2 * kRawBytes, kPartStage = 6 * kPartBytes;
+constexpr int kSplitSmem = kRawStages * kRawStage + kPartStages * kPartStage + 1024;
+constexpr int kSumSlices = 512 / kSlice;     // slices accumulated in TMEM at a time
+constexpr int kConvertWarps = 8;
+
+struct SplitParams {
+  CUtensorMap map_x, map_w, map_up;
+  Problem p;
+  int box_m;   // activation rows copied and split per slice
+  int w_mn;    // weights with the output features contiguous
+  int splits;  // CTAs per tile
+  int row_tiles;
+  int vec;     // four neighbouring outputs are one 16-byte store
+};
+
+// Eight fp32 numbers as 3 x 8 bf16, packed in 16 bytes each.
+__device__ __forceinline__ void split8(const float4& a, const float4& b, uint4 (&part)[3]) {
+  const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  uint32_t h[8], m[8], l[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t bits = __float_as_uint(x[e]);
+    const bool special = (bits & 0x7f800000u) == 0x7f800000u;
+    h[e] = bits & 0xffff0000u;
+    if (special && (bits & 0x007fffffu)) h[e] = 0x7fc00000u;  // NaN, wherever its bits are
+    const float r = special ? 0.f : x[e] - __uint_as_float(h[e]);
+    m[e] = __float_as_uint(r) & 0xffff0000u;
+    l[e] = __float_as_uint(r - __uint_as_float(m[e]));
+  }
+  auto pack = [](const uint32_t (&v)[8]) {  // the upper halves of neighbours
+    return make_uint4(__byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632),
+                      __byte_perm(v[4], v[5], 0x7632), __byte_perm(v[6], v[7], 0x7632));
+  };
+  part[0] = pack(h);
+  part[1] = pack(m);
+  part[2] = pack(l);
+}
+
+// 64-byte-swizzled K-major tile: rows of 32 bf16, atoms of 8 rows.
+__device__ __forceinline__ uint64_t smem_desc_sw64(uint32_t addr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((addr >> 4) & 0x3fff);
+  d |= static_cast<uint64_t>(1) << 16;            // leading dimension: not used K-major
+  d |= static_cast<uint64_t>(512 >> 4) << 32;     // between atoms
+  d |= static_cast<uint64_t>(1) << 46;            // version: sm_100
+  d |= static_cast<uint64_t>(4) << 61;            // 64-byte swizzle
+  return d;
+}
+
+// x[row] . w[n] in fp32 multiply-adds.
+__device__ __noinline__ float plain_dot(const Problem& p, const float* w, int row, int n) {
+  const float* x = static_cast<const float*>(p.x) + row * p.x_rs;
+  w += n * p.w_ns;
+  float y = 0.f;
+  for (int k = 0; k < p.inner; ++k) y = fmaf(x[k], w[k * p.w_ks], y);
+  return y;
+}
+
+template <typename T, Kind kKind, int kAct>
+__global__ void __launch_bounds__(kSplitThreads, 1)
+    split_kernel(const __grid_constant__ SplitParams g) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t raw_full[kRawStages], raw_empty[kRawStages];
+  __shared__ uint64_t part_full[kPartStages], part_empty[kPartStages];
+  __shared__ uint64_t acc_full[2], acc_empty[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int aborted;
+  constexpr int kSet = kKind == kGated ? kTile / 2 : kTile;  // output features per tile
+  const Problem& p = g.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* raw = smem;
+  uint8_t* parts = smem + kRawStages * kRawStage;
+  const int rank = g.splits > 1 ? static_cast<int>(tc::cluster_rank()) : 0;
+  const int tile = blockIdx.x / g.splits;
+  const int m0 = tile % g.row_tiles * kTile;
+  const int n0 = tile / g.row_tiles * kSet;
+  const int slices = (p.inner + kSlice - 1) / kSlice;
+  const int first = static_cast<int>(static_cast<int64_t>(slices) * rank / g.splits);
+  const int count = static_cast<int>(static_cast<int64_t>(slices) * (rank + 1) / g.splits) - first;
+
+  if (threadIdx.x == 0) {
+    tc::prefetch_tensormap(&g.map_x);
+    tc::prefetch_tensormap(&g.map_w);
+    if (kKind == kGated) tc::prefetch_tensormap(&g.map_up);
+    for (int i = 0; i < kRawStages; ++i) {
+      tc::mbar_init(&raw_full[i], 1);
+      tc::mbar_init(&raw_empty[i], kConvertWarps);
+    }
+    for (int i = 0; i < kPartStages; ++i) {
+      tc::mbar_init(&part_full[i], kConvertWarps);
+      tc::mbar_init(&part_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&acc_full[i], 1);
+      tc::mbar_init(&acc_empty[i], 8);
+    }
+    aborted = 0;
+    tc::fence_mbar_init();
+  }
+  if (warp == 17) tc::tmem_alloc(&tmem_slot, 512);
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  tc::pdl_launch_dependents();
+  tc::pdl_wait();
+  const uint32_t tmem = tmem_slot;
+  bool ok = true;
+  float v[64];  // warps 0-7: this thread's row, half of the columns
+
+  if (warp == 16) {
+    const uint32_t bytes = kRawBytes + g.box_m * 128;
+    Ring at;
+    for (int i = 0; i < count; ++i, at.next(kRawStages)) {
+      if (!__all_sync(kFullMask, tc::mbar_wait(&raw_empty[at.slot], at.parity ^ 1, kWaitLimit))) {
+        ok = false;
+        break;
+      }
+      if (tc::elect_one()) {
+        uint64_t* bar = &raw_full[at.slot];
+        uint8_t* x = raw + at.slot * kRawStage;
+        uint8_t* w = x + kRawBytes;
+        const int k0 = (first + i) * kSlice;
+        tc::mbar_expect_tx(bar, bytes);
+        tc::tma_load_2d(x, &g.map_x, bar, k0, m0);
+        if (g.w_mn) {  // boxes of 32 output features by 32 input features
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            const bool second = kKind == kGated && b >= 2;
+            tc::tma_load_2d(w + b * 4096, second ? &g.map_up : &g.map_w, bar,
+                            n0 + b * 32 - (second ? kSet : 0), k0);
+          }
+        } else {
+          tc::tma_load_2d(w, &g.map_w, bar, k0, n0);
+          if (kKind == kGated) tc::tma_load_2d(w + kRawBytes / 2, &g.map_up, bar, k0, n0);
+        }
+      }
+      __syncwarp();
+    }
+  } else if (warp == 17) {
+    const uint32_t idesc = tc::idesc_f16(1, kTile, kTile, g.w_mn);
+    const uint64_t x_desc = smem_desc_sw64(tc::smem_u32(parts));
+    const uint64_t w_desc = g.w_mn ? tc::smem_desc_sw128(tc::smem_u32(parts) + 3 * kPartBytes, 4096, 1024)
+                                   : smem_desc_sw64(tc::smem_u32(parts) + 3 * kPartBytes);
+    const uint32_t x_hi = static_cast<uint32_t>(x_desc >> 32);
+    const uint32_t w_hi = static_cast<uint32_t>(w_desc >> 32);
+    const uint32_t kstep_w = (g.w_mn ? 2048 : 32) >> 4;
+    Ring at, acc;
+    for (int i = 0; ok && i < count; acc.next(2)) {
+      if (!__all_sync(kFullMask, tc::mbar_poll(&acc_empty[acc.slot], acc.parity ^ 1, kWaitLimit))) {
+        ok = false;
+        break;
+      }
+      tc::tc_fence_after();
+      const uint32_t d = tmem + acc.slot * 256;
+      const int end = min(i + kSumSlices, count);
+      for (uint32_t more = 0; i < end; ++i, at.next(kPartStages)) {
+        if (!__all_sync(kFullMask, tc::mbar_poll(&part_full[at.slot], at.parity, kWaitLimit))) {
+          ok = false;
+          break;
+        }
+        tc::tc_fence_after();
+        if (tc::elect_one()) {
+          const uint32_t x_lo = static_cast<uint32_t>(x_desc) + at.slot * (kPartStage >> 4);
+          const uint32_t w_lo = static_cast<uint32_t>(w_desc) + at.slot * (kPartStage >> 4);
+          auto product = [&](uint32_t acc_at, int xp, int wp, int ks, uint32_t accumulate) {
+            tc::mma_f16_ss(acc_at, tc::desc64(x_lo + xp * (kPartBytes >> 4) + ks * 2, x_hi),
+                           tc::desc64(w_lo + wp * (kPartBytes >> 4) + ks * kstep_w, w_hi), idesc,
+                           accumulate);
+          };
+#pragma unroll
+          for (int ks = 0; ks < kSlice / 16; ++ks) {
+            const uint32_t go = ks > 0 ? 1 : more;
+            product(d, 0, 0, ks, go);
+            product(d + kTile, 0, 2, ks, go);
+            product(d + kTile, 2, 0, ks, 1);
+            product(d + kTile, 1, 1, ks, 1);
+            product(d + kTile, 0, 1, ks, 1);
+            product(d + kTile, 1, 0, ks, 1);
+          }
+          tc::mma_commit(&part_empty[at.slot]);
+          if (i == end - 1) tc::mma_commit(&acc_full[acc.slot]);
+        }
+        more = 1;
+        __syncwarp();
+      }
+    }
+  } else if (warp >= 8) {
+    // 16-byte units: lanes take neighbouring lines (rows, or input features of
+    // an MN-major slice), which keeps reads and writes free of bank conflicts
+    const int cw = warp - 8;
+    Ring at_raw, at_part;
+    for (int i = 0; i < count; ++i, at_raw.next(kRawStages), at_part.next(kPartStages)) {
+      ok = __all_sync(kFullMask,
+                      tc::mbar_wait(&raw_full[at_raw.slot], at_raw.parity, kWaitLimit) &&
+                          tc::mbar_wait(&part_empty[at_part.slot], at_part.parity ^ 1, kWaitLimit));
+      if (!ok) break;
+      const uint8_t* src = raw + at_raw.slot * kRawStage;
+      uint8_t* dst = parts + at_part.slot * kPartStage;
+      auto k_major = [&](const uint8_t* from, uint8_t* to, int rows) {
+        for (int u = cw; u < (rows + 31) / 32 * 4; u += kConvertWarps) {
+          const int row = u / 4 * 32 + lane, c = u % 4;
+          if (row < rows) {
+            const uint8_t* r = from + row * 128;
+            uint4 part[3];
+            split8(*reinterpret_cast<const float4*>(r + (((2 * c) ^ (row & 7)) << 4)),
+                   *reinterpret_cast<const float4*>(r + (((2 * c + 1) ^ (row & 7)) << 4)), part);
+            uint8_t* t = to + row * 64 + ((c ^ ((row >> 1) & 3)) << 4);
+#pragma unroll
+            for (int q = 0; q < 3; ++q) *reinterpret_cast<uint4*>(t + q * kPartBytes) = part[q];
+          }
+        }
+      };
+      k_major(src, dst, g.box_m);
+      if (g.w_mn) {
+        for (int u = cw; u < kTile / 8; u += kConvertWarps) {  // 8 output features, lane = k
+          const uint8_t* r = src + kRawBytes + u / 4 * 4096 + lane * 128;
+          const int c = u % 4;
+          uint4 part[3];
+          split8(*reinterpret_cast<const float4*>(r + (((2 * c) ^ (lane & 7)) << 4)),
+                 *reinterpret_cast<const float4*>(r + (((2 * c + 1) ^ (lane & 7)) << 4)), part);
+          uint8_t* t = dst + 3 * kPartBytes + u / 8 * 4096 + lane * 128 +
+                       (((u & 7) ^ (lane & 7)) << 4);
+#pragma unroll
+          for (int q = 0; q < 3; ++q) *reinterpret_cast<uint4*>(t + q * kPartBytes) = part[q];
+        }
+      } else {
+        k_major(src + kRawBytes, dst + 3 * kPartBytes, kTile);
+      }
+      tc::fence_proxy_async_smem();  // the parts are read by the tensor core
+      __syncwarp();
+      if (lane == 0) {
+        tc::mbar_arrive(&part_full[at_part.slot]);
+        tc::mbar_arrive(&raw_empty[at_raw.slot]);
+      }
+    }
+  } else {
+    const uint32_t taddr = tmem + (static_cast<uint32_t>(warp & 3) << 21) + (warp >> 2) * 64;
+    Ring acc;
+    for (int i = 0; i < count; i += kSumSlices, acc.next(2)) {
+      ok = __all_sync(kFullMask, tc::mbar_wait(&acc_full[acc.slot], acc.parity, kWaitLimit));
+      if (!ok) break;
+      tc::tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < 64; c += 16) {
+        uint32_t big[16], small[16];
+        tc::tmem_ld16(taddr + acc.slot * 256 + c, big);
+        tc::tmem_ld16(taddr + acc.slot * 256 + kTile + c, small);
+        tc::tmem_ld_wait(big);
+        tc::tmem_ld_wait(small);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float t = __uint_as_float(big[j]) + __uint_as_float(small[j]);
+          v[c + j] = i == 0 ? t : v[c + j] + t;
+        }
+      }
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&acc_empty[acc.slot]);
+    }
+  }
+  if (!ok) {  // a wait ran out: let copies in flight land before the memory goes
+    aborted = 1;
+    const long long start = clock64();
+    while (clock64() - start < 4000000LL) {
+    }
+  }
+  __syncwarp();
+
+  const int half = warp >> 2;
+  if constexpr (kKind == kVocab) {
+    if (warp < 8) {
+      const int row = m0 + (warp & 3) * 32 + lane, at = n0 + half * 64;
+      const int cols = min(64, p.outer - at);
+      bool odd = false;
+#pragma unroll
+      for (int j = 0; j < 64; ++j) odd = odd || (j < cols && v[j] != v[j]);
+      if (odd && row < p.rows) {
+#pragma unroll
+        for (int j = 0; j < 64; ++j)
+          if (j < cols && v[j] != v[j])
+            v[j] = plain_dot(p, static_cast<const float*>(p.w), row, at + j);
+      }
+      __syncwarp();
+      const int64_t want = p.tokens != nullptr && row < p.rows ? p.tokens[row] : -1;
+      const VocabPart part = vocab_part<64>(p, v, at, cols, want);
+      if (row < p.rows)
+        *reinterpret_cast<float4*>(
+            &p.parts[static_cast<int64_t>(row) * p.tiles + tile / g.row_tiles * 2 + half]) =
+            make_float4(part.most, part.sum, __int_as_float(part.at), part.chosen);
+    }
+  } else {
+    // every role is done with the stages: the sums take their place, rows of
+    // 128 columns (gate then up) in 16-byte units swizzled by row
+    __syncthreads();
+    if (warp < 8) {
+      const int r = (warp & 3) * 32 + lane;
+#pragma unroll
+      for (int c = 0; c < 16; ++c)
+        *reinterpret_cast<float4*>(smem + r * 512 + (((half * 16 + c) ^ (r & 7)) << 4)) =
+            make_float4(v[c * 4], v[c * 4 + 1], v[c * 4 + 2], v[c * 4 + 3]);
+    }
+    if (g.splits > 1)
+      tc::cluster_sync();
+    else
+      __syncthreads();
+    // Each CTA of the cluster finishes every splits-th row, adding in rank order.
+    constexpr int kLanes = kSet / 4;  // lanes per row, four features each
+    const int c = lane % kLanes, n = n0 + c * 4;
+    const int rows = min(kTile, p.rows - m0);
+    if (n < p.outer) {
+      const float* bias_at = static_cast<const float*>(p.bias);
+      const float* res_at = static_cast<const float*>(p.residual);
+      float bias[4];
+      read4<float>(bias_at != nullptr ? bias_at + n : nullptr, p.outer - n, bias);
+      constexpr int kRowsPerPass = kSplitThreads / kLanes;
+      for (int r = rank + (warp * (32 / kLanes) + lane / kLanes) * g.splits; r < rows;
+           r += kRowsPerPass * g.splits) {
+        float add[4];
+        read4<float>(res_at != nullptr ? res_at + (m0 + r) * p.r_rs + n : nullptr, p.outer - n, add);
+        float y[2][4];
+#pragma unroll
+        for (int op = 0; op < (kKind == kGated ? 2 : 1); ++op) {
+          const uint8_t* at = smem + r * 512 + (((op * 16 + c) ^ (r & 7)) << 4);
+          float4 t[kMaxSplits];
+#pragma unroll
+          for (int s = 0; s < kMaxSplits; ++s)
+            if (s < g.splits)
+              t[s] = g.splits > 1 ? tc::ld_peer4(tc::peer_smem(at, s))
+                                  : *reinterpret_cast<const float4*>(at);
+#pragma unroll
+          for (int s = 1; s < kMaxSplits; ++s)
+            if (s < g.splits) {
+              t[0].x += t[s].x;
+              t[0].y += t[s].y;
+              t[0].z += t[s].z;
+              t[0].w += t[s].w;
+            }
+          y[op][0] = t[0].x;
+          y[op][1] = t[0].y;
+          y[op][2] = t[0].z;
+          y[op][3] = t[0].w;
+          const float* w = static_cast<const float*>(op == 0 ? p.w : p.w_up);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (y[op][e] != y[op][e] && n + e < p.outer)
+              y[op][e] = plain_dot(p, w, m0 + r, n + e);
+        }
+        finish4<float, kKind, kAct>(p, g.vec, m0 + r, n, y[0], y[kKind == kGated ? 1 : 0], bias,
+                                    add);
+      }
+    }
+  }
+  __syncwarp();
+  tc::tc_fence_before();
+  if (g.splits > 1)
+    tc::cluster_sync();  // a peer may still be reading this CTA's sums
+  else
+    __syncthreads();
+  if (aborted && threadIdx.x == 0) raise_status(p.status, kStatusTimeout);
+  if (warp == 17) {
+    tc::tc_fence_after();
+    tc::tmem_dealloc(tmem, 512);
+  }
+}
+
+template <typename T, Kind kKind, int kAct>
+int launch(const SplitParams& g, int ctas, cudaStream_t stream) {
+  constexpr auto kernel = split_kernel<T, kKind, kAct>;
+  if (const cudaError_t e = allow_smem<kernel>(kSplitSmem)) return static_cast<int>(e);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.blockDim = dim3(kSplitThreads);
+  cfg.dynamicSmemBytes = kSplitSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attrs[2];
+  cfg.attrs = attrs;
+  cfg.numAttrs = launch_attributes(attrs, g.splits);
+  return launch_status(cudaLaunchKernelEx(&cfg, kernel, g));
+}
+
+}  // namespace
+
+int split_vocab_parts(const Problem& p) { return 2 * ceil_div(p.outer, kTile); }
+
+int run_split(Kind kind, const Problem& p, int ctas, cudaStream_t stream) {
+  SplitParams g{};
+  const int set = kind == kGated ? kTile / 2 : kTile;
+  g.p = p;
+  g.w_mn = p.w_ks != 1;
+  g.row_tiles = ceil_div(p.rows, kTile);
+  g.box_m = p.rows >= kTile ? kTile : ceil_div(p.rows, 8) * 8;
+  const int64_t tiles = static_cast<int64_t>(g.row_tiles) * ceil_div(p.outer, set);
+  const int slices = ceil_div(p.inner, kSlice);
+  // one CTA fits an SM; each takes at least four slices
+  g.splits = 1;
+  while (kind != kVocab && g.splits < kMaxSplits && slices >= 4 * (g.splits + 1) &&
+         tiles * (g.splits + 1) <= ctas)
+    ++g.splits;
+  if (tiles * g.splits > INT32_MAX) return RLT_E_SHAPE;
+  g.vec = p.outer % 4 == 0 && p.o_rs % 4 == 0 && aligned_to(p.out, 16);
+  bool ok = encode2d(&g.map_x, RLT_F32, p.x, p.inner, p.rows, p.x_rs, g.box_m);
+  for (int op = 0; op < (kind == kGated ? 2 : 1); ++op) {
+    CUtensorMap* map = op ? &g.map_up : &g.map_w;
+    const void* base = op ? p.w_up : p.w;
+    ok = ok && (g.w_mn ? encode2d(map, RLT_F32, base, p.outer, p.inner, p.w_ks, kSlice)
+                       : encode2d(map, RLT_F32, base, p.inner, p.outer, p.w_ns, set));
+  }
+  if (!ok) return RLT_E_DEVICE;
+  const int grid = static_cast<int>(tiles * g.splits);
+  switch (kind) {
+    case kLinear: return by_activation<kLinear, float>(g, grid, stream);
+    case kGated: return by_activation<kGated, float>(g, grid, stream);
+    default: return by_activation<kVocab, float>(g, grid, stream);
+  }
+}
+
+}  // namespace proj
+}  // namespace rlt

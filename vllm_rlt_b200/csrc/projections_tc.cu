@@ -30,19 +30,12 @@
 // 64 columns): a CTA streams 128 output features over its share of the input
 // features, a cluster of up to 8 CTAs shares a feature tile, and their partial
 // sums meet in distributed shared memory.
-#include <cuda.h>
-#include <cudaTypedefs.h>
-
-#include <atomic>
-
-#include "proj_common.cuh"
-#include "tc_ptx.cuh"
+#include "proj_tc.cuh"
 
 namespace rlt {
 namespace proj {
 namespace {
 
-constexpr long long kWaitLimit = 100000000LL;  // cycles (~50 ms)
 constexpr int kBlockK = 64;                    // input features per stage (128 bytes)
 constexpr int kTileM = 128;                    // activation rows per CTA
 constexpr int kMaxStages = 10;
@@ -54,7 +47,6 @@ constexpr int kLaunchRegs = 168, kSumRegs = 232, kOtherRegs = 40;  // per thread
 static_assert(256 * kSumRegs + 128 * kOtherRegs <= kThreads * kLaunchRegs,
               "the increase draws on what the launch allocated");
 constexpr int kStagingBytes = kEpilogueWarps * 4096;  // 32 rows x 32 fp32 columns per warp
-constexpr int kSmemBudget = 224 * 1024;               // dynamic shared memory of a CTA
 constexpr int kVocabBlocks = 8;  // 64-feature blocks accumulated in TMEM at a time by the head
 
 struct GemmParams {
@@ -74,20 +66,6 @@ struct GemmParams {
   int pair;       // tiles of 256 rows on pairs of CTAs
 };
 
-// Position in a ring of barriers: a slot, and the parity its next use has. The
-// issuing threads step it without divisions (with them a 64-feature block took
-// them 570 and 740 cycles, more than its 512 of arithmetic).
-struct Ring {
-  int slot = 0;
-  uint32_t parity = 0;
-  __device__ __forceinline__ void next(int size) {
-    if (++slot == size) {
-      slot = 0;
-      parity ^= 1;
-    }
-  }
-};
-
 template <typename T>
 struct Fmt;
 template <>
@@ -98,19 +76,6 @@ template <>
 struct Fmt<__nv_bfloat16> {
   static constexpr uint32_t value = 1;
 };
-
-// Four neighbouring 16-bit values (8-byte aligned in memory).
-template <typename T>
-__device__ __forceinline__ void widen4(const uint2& r, float (&v)[4]) {
-  T t[4];
-  *reinterpret_cast<uint2*>(t) = r;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = to_f32<T>(t[e]);
-}
-template <typename T>
-__device__ __forceinline__ void load4(const T* p, float (&v)[4]) {
-  widen4<T>(*reinterpret_cast<const uint2*>(p), v);
-}
 
 // Columns n .. n + 31 of a warp's 32 rows, from the threads' registers (one row
 // each) to `out`: the values go through shared memory so that neighbouring
@@ -180,52 +145,6 @@ __device__ __forceinline__ void finish32(const Problem& p, int vec, uint8_t* sta
   __syncwarp();
 }
 
-// A thread's record of its columns v[0 .. cols) of one vocabulary tile, the
-// first of them vocabulary entry n0.
-__device__ __forceinline__ VocabPart vocab_part(const Problem& p, const float (&v)[128], int n0,
-                                                int cols, int64_t want) {
-  VocabPart part{-INFINITY, 0.f, INT32_MAX, 0.f};
-  if (cols <= 0) return part;
-#pragma unroll
-  for (int c = 0; c < 128; c += 16)
-    if (c < cols)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) part.most = fmaxf(part.most, c + j < cols ? v[c + j] : -INFINITY);
-  const float base = part.most == -INFINITY ? 0.f : part.most;
-  float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-  for (int c = 0; c < 128; c += 16)
-    if (c < cols)
-#pragma unroll
-      for (int j = 0; j < 16; j += 2) {
-        s0 += c + j < cols ? ex2((v[c + j] - base) * kLog2e) : 0.f;
-        s1 += c + j + 1 < cols ? ex2((v[c + j + 1] - base) * kLog2e) : 0.f;
-      }
-  part.sum = s0 + s1;
-  if (p.tokens != nullptr) {
-    const bool here = want >= n0 && want < n0 + cols;
-    if (__any_sync(kFullMask, here)) {
-      const int at = here ? static_cast<int>(want - n0) : -1;
-#pragma unroll
-      for (int j = 0; j < 128; ++j)
-        if (j == at) part.chosen = v[j];
-    }
-    return part;
-  }
-#pragma unroll
-  for (int j = 127; j >= 0; --j)
-    if (j < cols && v[j] == part.most) part.at = n0 + j;
-  if (__any_sync(kFullMask, part.sum != part.sum)) {  // a NaN counts as the largest: the first
-#pragma unroll
-    for (int j = 127; j >= 0; --j)
-      if (j < cols && v[j] != v[j]) {
-        part.most = v[j];
-        part.at = n0 + j;
-      }
-  }
-  return part;
-}
-
 template <typename T, Kind kKind, int kAct, bool kPair>
 __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant__ GemmParams g) {
   extern __shared__ uint8_t smem_raw[];
@@ -267,6 +186,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
   else
     __syncthreads();
   tc::tc_fence_after();
+  tc::pdl_launch_dependents();
+  tc::pdl_wait();
   const uint32_t tmem = tmem_slot;
 
   const int kblocks = (p.inner + kBlockK - 1) / kBlockK;
@@ -486,7 +407,6 @@ constexpr int kStreamThreads = 192;
 constexpr int kStreamRows = 64;     // activation rows that stream_kernel takes
 constexpr int kStreamStages = 12;
 constexpr int kStreamFeatures = 128;
-constexpr int kMaxSplits = 8;       // CTAs of a cluster (the portable limit)
 
 struct StreamParams {
   CUtensorMap map_x, map_w, map_up;
@@ -534,6 +454,8 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
+  tc::pdl_launch_dependents();
+  tc::pdl_wait();
   const uint32_t tmem = tmem_slot;
   bool ok = true;
 
@@ -639,18 +561,13 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
   const int n = n0 + f0;
   if (n < p.outer) {
     const T* res = static_cast<const T*>(p.residual);
-    float b[4] = {0.f, 0.f, 0.f, 0.f};
-    if (kKind == kLinear && p.bias != nullptr)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (n + e < p.outer) b[e] = to_f32<T>(static_cast<const T*>(p.bias)[n + e]);
+    const T* bias = static_cast<const T*>(p.bias);
+    float b[4];
+    read4<T>(bias != nullptr ? bias + n : bias, p.outer - n, b);
 #pragma unroll 2
     for (int row = rank + warp * g.splits; row < p.rows; row += kStreamThreads / 32 * g.splits) {
-      float r[4] = {0.f, 0.f, 0.f, 0.f};
-      if (kKind == kLinear && res != nullptr)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (n + e < p.outer) r[e] = to_f32<T>(res[row * p.r_rs + n + e]);
+      float r[4];
+      read4<T>(res != nullptr ? res + row * p.r_rs + n : res, p.outer - n, r);
       float y[kOps][4];
 #pragma unroll
       for (int op = 0; op < kOps; ++op) {
@@ -674,22 +591,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
         y[op][2] = t.z;
         y[op][3] = t.w;
       }
-      T o[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if constexpr (kKind == kGated)
-          o[e] = from_f32<T>(activate<false, kAct>(y[0][e]) * y[1][e]);
-        else
-          o[e] = from_f32<T>(activate<false, kAct>(y[0][e] + b[e]) + r[e]);
-      }
-      T* out = static_cast<T*>(p.out) + row * p.o_rs + n;
-      if (g.vec) {
-        *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(o);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (n + e < p.outer) out[e] = o[e];
-      }
+      finish4<T, kKind, kAct>(p, g.vec, row, n, y[0], y[kOps - 1], b, r);
     }
   }
   if (g.splits > 1) {
@@ -700,56 +602,6 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
 
 // ---- host side --------------------------------------------------------------
 
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  static std::atomic<void*> known{nullptr};
-  void* fn = known.load();
-  if (fn == nullptr) {
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) !=
-            cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      return nullptr;
-    known.store(fn);
-  }
-  return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
-}
-
-// A [lines x line] matrix of 16-bit elements, `stride` elements between lines,
-// copied in boxes of 64 elements by `box_lines` lines.
-bool encode2d(CUtensorMap* map, int32_t dtype, const void* base, int line, int lines,
-              int64_t stride, int box_lines) {
-  auto fn = encode_fn();
-  if (fn == nullptr) return false;
-  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(line), static_cast<cuuint64_t>(lines)};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride) * 2};
-  const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(box_lines)};
-  const cuuint32_t elem[2] = {1, 1};
-  return fn(map,
-            dtype == RLT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-            2, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-// Dynamic shared memory of kKernel raised (and its register count checked) once
-// per device.
-template <auto kKernel>
-cudaError_t allow_smem(int bytes, int least_regs = 0) {
-  static std::atomic<bool> done[64];
-  int dev = 0;
-  if (const cudaError_t e = cudaGetDevice(&dev)) return e;
-  if (dev >= 0 && dev < 64 && done[dev].load()) return cudaSuccess;
-  cudaError_t e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess && least_regs > 0) {
-    // with fewer registers at launch a warpgroup's increase could never be granted
-    cudaFuncAttributes attr{};
-    e = cudaFuncGetAttributes(&attr, kKernel);
-    if (e == cudaSuccess && attr.numRegs < least_regs) e = cudaErrorInvalidConfiguration;
-  }
-  if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev].store(true);
-  return e;
-}
-
 template <typename T, Kind kKind, int kAct>
 int launch(const GemmParams& g, int ctas, cudaStream_t stream) {
   const int regs = kKind == kVocab ? kLaunchRegs : 0;
@@ -758,12 +610,9 @@ int launch(const GemmParams& g, int ctas, cudaStream_t stream) {
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = kStagingBytes + g.ring_bytes + 1024;
   cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = g.pair ? 2 : 1;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attrs[2];
+  cfg.attrs = attrs;
+  cfg.numAttrs = launch_attributes(attrs, g.pair ? 2 : 1);
   if (g.pair) {
     constexpr auto kernel = gemm_kernel<T, kKind, kAct, true>;
     if (const cudaError_t e = allow_smem<kernel>(kSmemBudget, regs)) return static_cast<int>(e);
@@ -773,8 +622,6 @@ int launch(const GemmParams& g, int ctas, cudaStream_t stream) {
   if (const cudaError_t e = allow_smem<kernel>(kSmemBudget, regs)) return static_cast<int>(e);
   return launch_status(cudaLaunchKernelEx(&cfg, kernel, g));
 }
-
-bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
 
 // How gemm_kernel tiles a problem: output features per tile, and whether a
 // tile is a pair of CTAs' (256 rows) or one CTA's (128).
@@ -827,31 +674,12 @@ int launch(const StreamParams& g, int tiles, cudaStream_t stream) {
   cfg.blockDim = dim3(kStreamThreads);
   cfg.dynamicSmemBytes = g.stages * g.stage_bytes + 1024;
   cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = g.splits;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attrs[2];
+  cfg.attrs = attrs;
+  cfg.numAttrs = launch_attributes(attrs, g.splits);
   return launch_status(cudaLaunchKernelEx(&cfg, kernel, g));
 }
 
-// The kernel for a launch's type and activation.
-template <Kind kKind, typename T, typename Params>
-int by_activation(const Params& g, int ctas, cudaStream_t stream) {
-  if constexpr (kKind == kVocab) {
-    return launch<T, kKind, RLT_ACT_NONE>(g, ctas, stream);
-  } else {
-    switch (g.p.act) {
-      case RLT_ACT_SILU: return launch<T, kKind, RLT_ACT_SILU>(g, ctas, stream);
-      case RLT_ACT_GELU: return launch<T, kKind, RLT_ACT_GELU>(g, ctas, stream);
-      case RLT_ACT_GELU_TANH: return launch<T, kKind, RLT_ACT_GELU_TANH>(g, ctas, stream);
-      case RLT_ACT_RELU: return launch<T, kKind, RLT_ACT_RELU>(g, ctas, stream);
-      case RLT_ACT_SIGMOID: return launch<T, kKind, RLT_ACT_SIGMOID>(g, ctas, stream);
-      default: return launch<T, kKind, RLT_ACT_NONE>(g, ctas, stream);
-    }
-  }
-}
 template <Kind kKind, typename Params>
 int by_type(const Params& g, int32_t dtype, int ctas, cudaStream_t stream) {
   return dtype == RLT_BF16 ? by_activation<kKind, __nv_bfloat16>(g, ctas, stream)
@@ -864,7 +692,7 @@ int run_stream(Kind kind, const Problem& p, int32_t dtype, int ctas, cudaStream_
   g.p = p;
   g.w_mn = p.w_ks != 1;
   g.cols = ceil_div(p.rows, 16) * 16;
-  g.vec = p.outer % 4 == 0 && p.o_rs % 4 == 0 && aligned8(p.out);
+  g.vec = p.outer % 4 == 0 && p.o_rs % 4 == 0 && aligned_to(p.out, 8);
   g.stage_bytes = ops * kStreamFeatures * kBlockK * 2 + g.cols * 128;
   const int tiles = ceil_div(p.outer, kStreamFeatures);
   const int kblocks = ceil_div(p.inner, kBlockK);
@@ -916,7 +744,7 @@ int run_tc(Kind kind, const Problem& p, int32_t dtype, int ctas, cudaStream_t st
   g.stages = (kSmemBudget - kStagingBytes - 1024 - (kTileM - g.box_m) * 128) / g.stage_bytes;
   if (g.stages > kMaxStages) g.stages = kMaxStages;
   g.ring_bytes = g.stages * g.stage_bytes + (kTileM - g.box_m) * 128;
-  g.vec = aligned8(p.out) && p.o_rs % 4 == 0 && aligned8(p.bias) && aligned8(p.residual) &&
+  g.vec = aligned_to(p.out, 8) && p.o_rs % 4 == 0 && aligned_to(p.bias, 8) && aligned_to(p.residual, 8) &&
           p.r_rs % 4 == 0;
   if (static_cast<int64_t>(g.row_tiles) * g.col_tiles > INT32_MAX) return RLT_E_SHAPE;
   bool ok = encode2d(&g.map_x, dtype, p.x, p.inner, p.rows, p.x_rs, g.box_m);

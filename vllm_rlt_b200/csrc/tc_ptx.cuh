@@ -102,6 +102,20 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, long l
   return true;
 }
 
+// ---- programmatic dependent launch ----------------------------------------
+//
+// A kernel launched with the programmatic serialisation attribute may start
+// while its predecessor in the stream still runs: its prologue (barriers,
+// TMEM, descriptors) then costs nothing. Nothing a predecessor may write, or
+// still read, is touched before pdl_wait, which returns once all of them have
+// completed and their writes are visible.
+__device__ __forceinline__ void pdl_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void pdl_launch_dependents() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 // One lane of a converged warp. The compiler knows the branch it guards to be
 // one thread's, so the TMA and tensor-core instructions in it take their
 // operands from uniform registers directly (behind a test of the lane number
