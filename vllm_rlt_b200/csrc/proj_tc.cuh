@@ -17,6 +17,13 @@ constexpr long long kWaitLimit = 100000000LL;  // cycles (~50 ms)
 constexpr int kMaxSplits = 8;                  // CTAs of a cluster (the portable limit)
 constexpr int kSmemBudget = 224 * 1024;        // dynamic shared memory of a CTA
 
+// The first 1024-byte boundary in dynamic shared memory, as an offset from it:
+// a pointer rounded up as a number would lose its address space, and every
+// access through it would be a generic one.
+__device__ __forceinline__ uint8_t* align_1024(uint8_t* smem) {
+  return smem + ((1024u - (tc::smem_u32(smem) & 1023u)) & 1023u);
+}
+
 // Position in a ring of barriers: a slot, and the parity its next use has. The
 // issuing threads step it without divisions (with them a 64-feature block took
 // them 570 and 740 cycles, more than its 512 of arithmetic).
@@ -44,6 +51,11 @@ __device__ __forceinline__ void load4(const T* p, float (&v)[4]) {
   widen4<T>(*reinterpret_cast<const uint2*>(p), v);
 }
 
+template <typename T>
+struct alignas(sizeof(T) * 4) Four {
+  T v[4];
+};
+
 // Four neighbouring outputs of a row from column n on: act(y + bias) +
 // residual, or act(y) * up. `vec`: they are one store (and all four exist).
 template <typename T, Kind kKind, int kAct>
@@ -51,9 +63,7 @@ __device__ __forceinline__ void finish4(const Problem& p, bool vec, int row, int
                                         const float (&y)[4], const float (&up)[4],
                                         const float (&bias)[4], const float (&add)[4]) {
   constexpr bool kPrecise = sizeof(T) == 4;
-  struct alignas(sizeof(T) * 4) Four {
-    T v[4];
-  } o;
+  Four<T> o;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     if constexpr (kKind == kGated)
@@ -63,7 +73,7 @@ __device__ __forceinline__ void finish4(const Problem& p, bool vec, int row, int
   }
   T* out = static_cast<T*>(p.out) + row * p.o_rs + n;
   if (vec) {
-    *reinterpret_cast<Four*>(out) = o;
+    *reinterpret_cast<Four<T>*>(out) = o;
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -71,11 +81,18 @@ __device__ __forceinline__ void finish4(const Problem& p, bool vec, int row, int
   }
 }
 
-// Four neighbouring values of a vector or a row, zeros past `left`.
+// Four neighbouring values of a vector or a row (in one load where `vec`),
+// zeros past `left` and without one.
 template <typename T>
-__device__ __forceinline__ void read4(const T* at, int left, float (&v)[4]) {
+__device__ __forceinline__ void read4(const T* at, bool vec, int left, float (&v)[4]) {
+  if (at != nullptr && vec) {
+    const Four<T> f = *reinterpret_cast<const Four<T>*>(at);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = at != nullptr && e < left ? to_f32<T>(at[e]) : 0.f;
+    for (int e = 0; e < 4; ++e) v[e] = to_f32<T>(f.v[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = at != nullptr && e < left ? to_f32<T>(at[e]) : 0.f;
+  }
 }
 
 // A thread's record of its columns v[0 .. cols) of one vocabulary tile, the

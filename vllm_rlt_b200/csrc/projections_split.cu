@@ -14,15 +14,15 @@
 // input features go into them, and those sums are added in registers, rounded
 // to nearest.
 //
-// Infinities: a part of an infinity times a part that is zero would be NaN where
-// fp32 arithmetic gives an infinity. Any NaN that comes out is recomputed by
-// fp32 multiply-adds from the operands, so both end up as they would there.
+// Infinities: splitting one leaves NaN parts, so its row or column comes out as
+// NaN. Any NaN that comes out is recomputed by fp32 multiply-adds from the
+// operands, so infinities and NaN end up as they would there.
 //
-// A CTA (18 warps) takes a tile of 128 rows by 128 weight rows over its share of
+// A CTA (16 warps) takes a tile of 128 rows by 128 weight rows over its share of
 // the input features; a cluster of up to 8 CTAs shares a tile when there are few.
-// Warp 16 copies slices of 32 input features (fp32, 128 bytes) by TMA, warps
-// 8-15 split them into parts in shared memory, warp 17 issues the products,
-// warps 0-7 gather the sums. Per slice of 128 x 128 shared memory moves 32 KB
+// Warp 14 copies slices of 32 input features (fp32, 128 bytes) by TMA, warps
+// 0-13 split them into parts in shared memory, warp 15 issues the products, and
+// warps 0-7 gather the sums between slices. Per slice of 128 x 128 shared memory moves 32 KB
 // in, 80 KB through the split and 96 KB into the tensor core, about 1660
 // cycles against 768 of arithmetic: that traffic bounds the kernel.
 #include "proj_tc.cuh"
@@ -31,7 +31,7 @@ namespace rlt {
 namespace proj {
 namespace {
 
-constexpr int kSplitThreads = 18 * 32;
+constexpr int kSplitThreads = 16 * 32;
 constexpr int kSlice = 32;                   // input features per slice
 constexpr int kTile = 128;                   // rows, and weight rows, of a tile
 constexpr int kRawBytes = kTile * 128;       // one operand's slice as it arrives
@@ -40,7 +40,7 @@ constexpr int kRawStages = 3, kPartStages = 2;
 constexpr int kRawStage = 2 * kRawBytes, kPartStage = 6 * kPartBytes;
 constexpr int kSplitSmem = kRawStages * kRawStage + kPartStages * kPartStage + 1024;
 constexpr int kSumSlices = 512 / kSlice;     // slices accumulated in TMEM at a time
-constexpr int kConvertWarps = 8;
+constexpr int kConvertWarps = 14, kCopyWarp = 14, kIssueWarp = 15;
 
 struct SplitParams {
   CUtensorMap map_x, map_w, map_up;
@@ -49,7 +49,7 @@ struct SplitParams {
   int w_mn;    // weights with the output features contiguous
   int splits;  // CTAs per tile
   int row_tiles;
-  int vec;     // four neighbouring outputs are one 16-byte store
+  int vec;     // four neighbouring outputs (biases, residuals) are 16 aligned bytes
 };
 
 // Eight fp32 numbers as 3 x 8 bf16, packed in 16 bytes each.
@@ -58,11 +58,8 @@ __device__ __forceinline__ void split8(const float4& a, const float4& b, uint4 (
   uint32_t h[8], m[8], l[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const uint32_t bits = __float_as_uint(x[e]);
-    const bool special = (bits & 0x7f800000u) == 0x7f800000u;
-    h[e] = bits & 0xffff0000u;
-    if (special && (bits & 0x007fffffu)) h[e] = 0x7fc00000u;  // NaN, wherever its bits are
-    const float r = special ? 0.f : x[e] - __uint_as_float(h[e]);
+    h[e] = __float_as_uint(x[e]) & 0xffff0000u;
+    const float r = x[e] - __uint_as_float(h[e]);
     m[e] = __float_as_uint(r) & 0xffff0000u;
     l[e] = __float_as_uint(r - __uint_as_float(m[e]));
   }
@@ -107,8 +104,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   constexpr int kSet = kKind == kGated ? kTile / 2 : kTile;  // output features per tile
   const Problem& p = g.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  uint8_t* smem = reinterpret_cast<uint8_t*>(
-      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* smem = align_1024(smem_raw);
   uint8_t* raw = smem;
   uint8_t* parts = smem + kRawStages * kRawStage;
   const int rank = g.splits > 1 ? static_cast<int>(tc::cluster_rank()) : 0;
@@ -138,7 +134,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     aborted = 0;
     tc::fence_mbar_init();
   }
-  if (warp == 17) tc::tmem_alloc(&tmem_slot, 512);
+  if (warp == kIssueWarp) tc::tmem_alloc(&tmem_slot, 512);
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
@@ -148,7 +144,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   bool ok = true;
   float v[64];  // warps 0-7: this thread's row, half of the columns
 
-  if (warp == 16) {
+  if (warp == kCopyWarp) {
     const uint32_t bytes = kRawBytes + g.box_m * 128;
     Ring at;
     for (int i = 0; i < count; ++i, at.next(kRawStages)) {
@@ -177,7 +173,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
       }
       __syncwarp();
     }
-  } else if (warp == 17) {
+  } else if (warp == kIssueWarp) {
     const uint32_t idesc = tc::idesc_f16(1, kTile, kTile, g.w_mn);
     const uint64_t x_desc = smem_desc_sw64(tc::smem_u32(parts));
     const uint64_t w_desc = g.w_mn ? tc::smem_desc_sw128(tc::smem_u32(parts) + 3 * kPartBytes, 4096, 1024)
@@ -225,61 +221,13 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
         __syncwarp();
       }
     }
-  } else if (warp >= 8) {
-    // 16-byte units: lanes take neighbouring lines (rows, or input features of
-    // an MN-major slice), which keeps reads and writes free of bank conflicts
-    const int cw = warp - 8;
-    Ring at_raw, at_part;
-    for (int i = 0; i < count; ++i, at_raw.next(kRawStages), at_part.next(kPartStages)) {
-      ok = __all_sync(kFullMask,
-                      tc::mbar_wait(&raw_full[at_raw.slot], at_raw.parity, kWaitLimit) &&
-                          tc::mbar_wait(&part_empty[at_part.slot], at_part.parity ^ 1, kWaitLimit));
-      if (!ok) break;
-      const uint8_t* src = raw + at_raw.slot * kRawStage;
-      uint8_t* dst = parts + at_part.slot * kPartStage;
-      auto k_major = [&](const uint8_t* from, uint8_t* to, int rows) {
-        for (int u = cw; u < (rows + 31) / 32 * 4; u += kConvertWarps) {
-          const int row = u / 4 * 32 + lane, c = u % 4;
-          if (row < rows) {
-            const uint8_t* r = from + row * 128;
-            uint4 part[3];
-            split8(*reinterpret_cast<const float4*>(r + (((2 * c) ^ (row & 7)) << 4)),
-                   *reinterpret_cast<const float4*>(r + (((2 * c + 1) ^ (row & 7)) << 4)), part);
-            uint8_t* t = to + row * 64 + ((c ^ ((row >> 1) & 3)) << 4);
-#pragma unroll
-            for (int q = 0; q < 3; ++q) *reinterpret_cast<uint4*>(t + q * kPartBytes) = part[q];
-          }
-        }
-      };
-      k_major(src, dst, g.box_m);
-      if (g.w_mn) {
-        for (int u = cw; u < kTile / 8; u += kConvertWarps) {  // 8 output features, lane = k
-          const uint8_t* r = src + kRawBytes + u / 4 * 4096 + lane * 128;
-          const int c = u % 4;
-          uint4 part[3];
-          split8(*reinterpret_cast<const float4*>(r + (((2 * c) ^ (lane & 7)) << 4)),
-                 *reinterpret_cast<const float4*>(r + (((2 * c + 1) ^ (lane & 7)) << 4)), part);
-          uint8_t* t = dst + 3 * kPartBytes + u / 8 * 4096 + lane * 128 +
-                       (((u & 7) ^ (lane & 7)) << 4);
-#pragma unroll
-          for (int q = 0; q < 3; ++q) *reinterpret_cast<uint4*>(t + q * kPartBytes) = part[q];
-        }
-      } else {
-        k_major(src + kRawBytes, dst + 3 * kPartBytes, kTile);
-      }
-      tc::fence_proxy_async_smem();  // the parts are read by the tensor core
-      __syncwarp();
-      if (lane == 0) {
-        tc::mbar_arrive(&part_full[at_part.slot]);
-        tc::mbar_arrive(&raw_empty[at_raw.slot]);
-      }
-    }
   } else {
+    // The next group's sums into v (warps 0-7).
     const uint32_t taddr = tmem + (static_cast<uint32_t>(warp & 3) << 21) + (warp >> 2) * 64;
     Ring acc;
-    for (int i = 0; i < count; i += kSumSlices, acc.next(2)) {
+    auto gather = [&](bool first_group) {
       ok = __all_sync(kFullMask, tc::mbar_wait(&acc_full[acc.slot], acc.parity, kWaitLimit));
-      if (!ok) break;
+      if (!ok) return;
       tc::tc_fence_after();
 #pragma unroll
       for (int c = 0; c < 64; c += 16) {
@@ -291,13 +239,63 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const float t = __uint_as_float(big[j]) + __uint_as_float(small[j]);
-          v[c + j] = i == 0 ? t : v[c + j] + t;
+          v[c + j] = first_group ? t : v[c + j] + t;
         }
       }
       tc::tc_fence_before();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&acc_empty[acc.slot]);
+      acc.next(2);
+    };
+    // A warp's unit is 32 lines of 8 elements. Neighbouring lanes take
+    // neighbouring lines (rows, or input features of an MN-major slice), which
+    // keeps reads and writes free of bank conflicts.
+    const int x_units = (g.box_m + 31) / 32 * 4, units = x_units + kTile / 8;
+    Ring at_raw, at_part;
+    int gathered = 0;  // slices whose sums are in v
+    for (int i = 0; i < count; ++i, at_raw.next(kRawStages), at_part.next(kPartStages)) {
+      ok = __all_sync(kFullMask,
+                      tc::mbar_wait(&raw_full[at_raw.slot], at_raw.parity, kWaitLimit) &&
+                          tc::mbar_wait(&part_empty[at_part.slot], at_part.parity ^ 1, kWaitLimit));
+      if (!ok) break;
+      const uint8_t* src = raw + at_raw.slot * kRawStage;
+      uint8_t* dst = parts + at_part.slot * kPartStage;
+      for (int u = warp; u < units; u += kConvertWarps) {
+        const bool of_x = u < x_units;
+        const int q = of_x ? u : u - x_units;
+        const uint8_t* r;  // the line's 128 bytes
+        uint8_t* t;
+        int line = lane, c = q & 3;
+        if (of_x || !g.w_mn) {
+          line += q / 4 * 32;
+          r = src + (of_x ? 0 : kRawBytes) + line * 128;
+          t = dst + (of_x ? 0 : 3 * kPartBytes) + line * 64 + ((c ^ ((line >> 1) & 3)) << 4);
+        } else {
+          r = src + kRawBytes + q / 4 * 4096 + line * 128;
+          t = dst + 3 * kPartBytes + q / 8 * 4096 + line * 128 + (((q & 7) ^ (line & 7)) << 4);
+        }
+        if (!of_x || line < g.box_m) {
+          uint4 part[3];
+          split8(*reinterpret_cast<const float4*>(r + (((2 * c) ^ (line & 7)) << 4)),
+                 *reinterpret_cast<const float4*>(r + (((2 * c + 1) ^ (line & 7)) << 4)), part);
+#pragma unroll
+          for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4*>(t + k * kPartBytes) = part[k];
+        }
+      }
+      tc::fence_proxy_async_smem();  // the parts are read by the tensor core
+      __syncwarp();
+      if (lane == 0) {
+        tc::mbar_arrive(&part_full[at_part.slot]);
+        tc::mbar_arrive(&raw_empty[at_raw.slot]);
+      }
+      // a group's products have long been issued two slices into the next one
+      if (warp < 8 && i == gathered + kSumSlices + 1) {
+        gather(gathered == 0);
+        if (!ok) break;
+        gathered += kSumSlices;
+      }
     }
+    for (; ok && warp < 8 && gathered < count; gathered += kSumSlices) gather(gathered == 0);
   }
   if (!ok) {  // a wait ran out: let copies in flight land before the memory goes
     aborted = 1;
@@ -352,12 +350,14 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
       const float* bias_at = static_cast<const float*>(p.bias);
       const float* res_at = static_cast<const float*>(p.residual);
       float bias[4];
-      read4<float>(bias_at != nullptr ? bias_at + n : nullptr, p.outer - n, bias);
+      read4<float>(bias_at != nullptr ? bias_at + n : nullptr, g.vec, p.outer - n, bias);
       constexpr int kRowsPerPass = kSplitThreads / kLanes;
+#pragma unroll 2
       for (int r = rank + (warp * (32 / kLanes) + lane / kLanes) * g.splits; r < rows;
            r += kRowsPerPass * g.splits) {
         float add[4];
-        read4<float>(res_at != nullptr ? res_at + (m0 + r) * p.r_rs + n : nullptr, p.outer - n, add);
+        read4<float>(res_at != nullptr ? res_at + (m0 + r) * p.r_rs + n : nullptr, g.vec,
+                     p.outer - n, add);
         float y[2][4];
 #pragma unroll
         for (int op = 0; op < (kKind == kGated ? 2 : 1); ++op) {
@@ -381,10 +381,12 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
           y[op][2] = t[0].z;
           y[op][3] = t[0].w;
           const float* w = static_cast<const float*>(op == 0 ? p.w : p.w_up);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (y[op][e] != y[op][e] && n + e < p.outer)
-              y[op][e] = plain_dot(p, w, m0 + r, n + e);
+          const float any = y[op][0] + y[op][1] + y[op][2] + y[op][3];
+          if (any != any) {
+            for (int e = 0; e < 4; ++e)
+              if (y[op][e] != y[op][e] && n + e < p.outer)
+                y[op][e] = plain_dot(p, w, m0 + r, n + e);
+          }
         }
         finish4<float, kKind, kAct>(p, g.vec, m0 + r, n, y[0], y[kKind == kGated ? 1 : 0], bias,
                                     add);
@@ -398,7 +400,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   else
     __syncthreads();
   if (aborted && threadIdx.x == 0) raise_status(p.status, kStatusTimeout);
-  if (warp == 17) {
+  if (warp == kIssueWarp) {
     tc::tc_fence_after();
     tc::tmem_dealloc(tmem, 512);
   }
@@ -438,7 +440,8 @@ int run_split(Kind kind, const Problem& p, int ctas, cudaStream_t stream) {
          tiles * (g.splits + 1) <= ctas)
     ++g.splits;
   if (tiles * g.splits > INT32_MAX) return RLT_E_SHAPE;
-  g.vec = p.outer % 4 == 0 && p.o_rs % 4 == 0 && aligned_to(p.out, 16);
+  g.vec = p.outer % 4 == 0 && p.o_rs % 4 == 0 && p.r_rs % 4 == 0 && aligned_to(p.out, 16) &&
+          aligned_to(p.bias, 16) && aligned_to(p.residual, 16);
   bool ok = encode2d(&g.map_x, RLT_F32, p.x, p.inner, p.rows, p.x_rs, g.box_m);
   for (int op = 0; op < (kind == kGated ? 2 : 1); ++op) {
     CUtensorMap* map = op ? &g.map_up : &g.map_w;

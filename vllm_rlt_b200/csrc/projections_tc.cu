@@ -155,8 +155,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
   const Problem& p = g.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = kPair ? static_cast<int>(tc::cluster_rank()) : 0;
-  uint8_t* smem = reinterpret_cast<uint8_t*>(
-      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* smem = align_1024(smem_raw);
   uint8_t* ring = smem + kStagingBytes;
 
   if (threadIdx.x == 0) {
@@ -416,7 +415,7 @@ struct StreamParams {
   int cols;    // activation rows rounded up to the instruction's 16
   int w_mn;
   int splits;  // CTAs per feature tile
-  int vec;     // four neighbouring outputs are one 8-byte store
+  int vec;     // four neighbouring outputs (biases, residuals) are 8 aligned bytes
 };
 
 template <typename T, Kind kKind, int kAct>
@@ -429,8 +428,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
   __shared__ volatile int aborted;
   const Problem& p = g.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  uint8_t* smem = reinterpret_cast<uint8_t*>(
-      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* smem = align_1024(smem_raw);
   const int rank = g.splits > 1 ? static_cast<int>(tc::cluster_rank()) : 0;
   const int n0 = blockIdx.x / g.splits * kStreamFeatures;
   const int kblocks = (p.inner + kBlockK - 1) / kBlockK;
@@ -563,11 +561,11 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
     const T* res = static_cast<const T*>(p.residual);
     const T* bias = static_cast<const T*>(p.bias);
     float b[4];
-    read4<T>(bias != nullptr ? bias + n : bias, p.outer - n, b);
+    read4<T>(bias != nullptr ? bias + n : bias, g.vec, p.outer - n, b);
 #pragma unroll 2
     for (int row = rank + warp * g.splits; row < p.rows; row += kStreamThreads / 32 * g.splits) {
       float r[4];
-      read4<T>(res != nullptr ? res + row * p.r_rs + n : res, p.outer - n, r);
+      read4<T>(res != nullptr ? res + row * p.r_rs + n : res, g.vec, p.outer - n, r);
       float y[kOps][4];
 #pragma unroll
       for (int op = 0; op < kOps; ++op) {
@@ -692,7 +690,8 @@ int run_stream(Kind kind, const Problem& p, int32_t dtype, int ctas, cudaStream_
   g.p = p;
   g.w_mn = p.w_ks != 1;
   g.cols = ceil_div(p.rows, 16) * 16;
-  g.vec = p.outer % 4 == 0 && p.o_rs % 4 == 0 && aligned_to(p.out, 8);
+  g.vec = p.outer % 4 == 0 && p.o_rs % 4 == 0 && p.r_rs % 4 == 0 && aligned_to(p.out, 8) &&
+          aligned_to(p.bias, 8) && aligned_to(p.residual, 8);
   g.stage_bytes = ops * kStreamFeatures * kBlockK * 2 + g.cols * 128;
   const int tiles = ceil_div(p.outer, kStreamFeatures);
   const int kblocks = ceil_div(p.inner, kBlockK);
