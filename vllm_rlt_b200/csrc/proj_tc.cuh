@@ -196,6 +196,36 @@ cudaError_t allow_smem(int bytes, int least_regs = 0) {
   return e;
 }
 
+// Clusters of `size` CTAs of kKernel that the device runs at once, each CTA
+// with `smem` bytes of dynamic shared memory. An SM group of the die need not
+// hold a whole number of clusters, so this can be well below CTAs / size.
+template <auto kKernel>
+int resident_clusters(int size, int threads, int smem) {
+  static std::atomic<int> known[64][kMaxSplits + 1];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 1;
+  if (dev >= 0 && dev < 64)
+    if (const int n = known[dev][size].load()) return n;
+  if (allow_smem<kKernel>(smem) != cudaSuccess) return 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(size);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = size;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kKernel, &cfg) != cudaSuccess || n < 1) {
+    (void)cudaGetLastError();
+    return 1;
+  }
+  if (dev >= 0 && dev < 64) known[dev][size].store(n);
+  return n;
+}
+
 // The kernel for a launch's activation.
 template <typename T, Kind kKind, int kAct, typename Params>
 int launch(const Params& g, int ctas, cudaStream_t stream);

@@ -41,6 +41,7 @@ constexpr int kRawStage = 2 * kRawBytes, kPartStage = 6 * kPartBytes;
 constexpr int kSplitSmem = kRawStages * kRawStage + kPartStages * kPartStage + 1024;
 constexpr int kSumSlices = 512 / kSlice;     // slices accumulated in TMEM at a time
 constexpr int kConvertWarps = 14, kCopyWarp = 14, kIssueWarp = 15;
+constexpr int kGroupWarps = kConvertWarps / 2;  // even slices, odd slices
 
 struct SplitParams {
   CUtensorMap map_x, map_w, map_up;
@@ -121,10 +122,10 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     if (kKind == kGated) tc::prefetch_tensormap(&g.map_up);
     for (int i = 0; i < kRawStages; ++i) {
       tc::mbar_init(&raw_full[i], 1);
-      tc::mbar_init(&raw_empty[i], kConvertWarps);
+      tc::mbar_init(&raw_empty[i], kGroupWarps);
     }
     for (int i = 0; i < kPartStages; ++i) {
-      tc::mbar_init(&part_full[i], kConvertWarps);
+      tc::mbar_init(&part_full[i], kGroupWarps);
       tc::mbar_init(&part_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -251,16 +252,21 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     // neighbouring lines (rows, or input features of an MN-major slice), which
     // keeps reads and writes free of bank conflicts.
     const int x_units = (g.box_m + 31) / 32 * 4, units = x_units + kTile / 8;
-    Ring at_raw, at_part;
+    // Two groups of warps take every other slice, each with a part stage of its
+    // own, so that one group's waits and fences lie under the other's work.
+    const int group = warp & 1, member = warp >> 1;
+    Ring at_raw;
+    if (group) at_raw.next(kRawStages);
+    uint32_t part_parity = 1;
     int gathered = 0;  // slices whose sums are in v
-    for (int i = 0; i < count; ++i, at_raw.next(kRawStages), at_part.next(kPartStages)) {
+    for (int i = group; i < count; i += 2) {
       ok = __all_sync(kFullMask,
                       tc::mbar_wait(&raw_full[at_raw.slot], at_raw.parity, kWaitLimit) &&
-                          tc::mbar_wait(&part_empty[at_part.slot], at_part.parity ^ 1, kWaitLimit));
+                          tc::mbar_wait(&part_empty[group], part_parity, kWaitLimit));
       if (!ok) break;
       const uint8_t* src = raw + at_raw.slot * kRawStage;
-      uint8_t* dst = parts + at_part.slot * kPartStage;
-      for (int u = warp; u < units; u += kConvertWarps) {
+      uint8_t* dst = parts + group * kPartStage;
+      for (int u = member; u < units; u += kGroupWarps) {
         const bool of_x = u < x_units;
         const int q = of_x ? u : u - x_units;
         const uint8_t* r;  // the line's 128 bytes
@@ -285,11 +291,14 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
       tc::fence_proxy_async_smem();  // the parts are read by the tensor core
       __syncwarp();
       if (lane == 0) {
-        tc::mbar_arrive(&part_full[at_part.slot]);
+        tc::mbar_arrive(&part_full[group]);
         tc::mbar_arrive(&raw_empty[at_raw.slot]);
       }
-      // a group's products have long been issued two slices into the next one
-      if (warp < 8 && i == gathered + kSumSlices + 1) {
+      part_parity ^= 1;
+      at_raw.next(kRawStages);
+      at_raw.next(kRawStages);
+      // these sums' last products were issued slices ago
+      if (warp < 8 && i >= gathered + kSumSlices + 2) {
         gather(gathered == 0);
         if (!ok) break;
         gathered += kSumSlices;
@@ -434,11 +443,19 @@ int run_split(Kind kind, const Problem& p, int ctas, cudaStream_t stream) {
   g.box_m = p.rows >= kTile ? kTile : ceil_div(p.rows, 8) * 8;
   const int64_t tiles = static_cast<int64_t>(g.row_tiles) * ceil_div(p.outer, set);
   const int slices = ceil_div(p.inner, kSlice);
-  // one CTA fits an SM; each takes at least four slices
+  // CTAs per tile: one CTA fits an SM, so what counts is how many clusters run
+  // at once. In slices' times; a CTA pays about eight for its start and end.
   g.splits = 1;
-  while (kind != kVocab && g.splits < kMaxSplits && slices >= 4 * (g.splits + 1) &&
-         tiles * (g.splits + 1) <= ctas)
-    ++g.splits;
+  int64_t least = INT64_MAX;
+  for (int s = 1; s <= (kind == kVocab ? 1 : kMaxSplits) && slices >= 4 * s; ++s) {
+    constexpr auto kernel = split_kernel<float, kLinear, RLT_ACT_NONE>;
+    const int64_t at_once = s == 1 ? ctas : resident_clusters<kernel>(s, kSplitThreads, kSplitSmem);
+    const int64_t cost = (tiles + at_once - 1) / at_once * (ceil_div(slices, s) + 8);
+    if (cost < least) {
+      least = cost;
+      g.splits = s;
+    }
+  }
   if (tiles * g.splits > INT32_MAX) return RLT_E_SHAPE;
   g.vec = p.outer % 4 == 0 && p.o_rs % 4 == 0 && p.r_rs % 4 == 0 && aligned_to(p.out, 16) &&
           aligned_to(p.bias, 16) && aligned_to(p.residual, 16);
