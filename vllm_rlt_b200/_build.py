@@ -1,9 +1,12 @@
 """Build the sm_100a shared library in-tree with nvcc (no JIT cache).
 
 ``python -m vllm_rlt_b200._build`` compiles every ``csrc/*.cu`` into
-``vllm_rlt_b200/_lib/librlt_b200.so``. Objects are rebuilt only when their
+``vllm_rlt_b200/_lib/librlt_b200.so``, and ``csrc/binding.cpp`` into the Python
+extension ``_rlt_torch.so`` beside it. Objects are rebuilt only when their
 source, a header or the flags changed. The library is plain C ABI
-(``include/rlt_b200.h``) with the CUDA runtime linked statically.
+(``include/rlt_b200.h``) with the CUDA runtime linked statically; the extension
+is the torch-facing entry of the operators that are called at sizes where a
+ctypes call costs more than the kernel.
 """
 
 from __future__ import annotations
@@ -14,6 +17,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PACKAGE = Path(__file__).resolve().parent
@@ -21,6 +25,7 @@ ROOT = PACKAGE.parent
 CSRC = PACKAGE / "csrc"
 OUT_DIR = PACKAGE / "_lib"
 LIB_NAME = "librlt_b200.so"
+BINDING_NAME = "_rlt_torch.so"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = [
     "-O3",
@@ -94,5 +99,40 @@ def build(verbose: bool = False) -> Path:
     return lib
 
 
+def build_binding(verbose: bool = False) -> Path:
+    """Compile and link the Python extension against the installed torch."""
+    import torch
+
+    build_dir = PACKAGE / "_build"
+    build_dir.mkdir(exist_ok=True)
+    source = CSRC / "binding.cpp"
+    root = Path(torch.__file__).resolve().parent
+    cuda_include = Path(nvcc()).resolve().parents[1] / "include"
+    includes = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include",
+                sysconfig.get_paths()["include"], cuda_include]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f"-I{ROOT / 'include'}", *(f"-isystem{p}" for p in includes), str(source),
+           f"-L{OUT_DIR}", f"-l:{LIB_NAME}", "-Wl,-rpath,$ORIGIN", f"-L{root / 'lib'}",
+           f"-Wl,-rpath,{root / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    h = hashlib.sha256(" ".join(cmd + [torch.__version__]).encode())
+    for part in (source, *sorted((ROOT / "include").glob("*.h"))):
+        h.update(part.read_bytes())
+    out = OUT_DIR / BINDING_NAME
+    stamp = build_dir / "binding.stamp"
+    if out.exists() and stamp.exists() and stamp.read_text() == h.hexdigest():
+        return out
+    tmp = OUT_DIR / f".{BINDING_NAME}.tmp"
+    result = subprocess.run([*cmd, "-o", str(tmp)], capture_output=True, text=True)
+    if result.returncode != 0:
+        raise RuntimeError(f"g++ failed for {source.name}:\n{result.stderr[-6000:]}")
+    os.replace(tmp, out)
+    stamp.write_text(h.hexdigest())
+    if verbose:
+        print(f"compiled {source.name}", file=sys.stderr)
+    return out
+
+
 if __name__ == "__main__":
     print(build(verbose=True))
+    print(build_binding(verbose=True))

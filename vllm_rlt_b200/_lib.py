@@ -9,18 +9,19 @@ route through another implementation.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import threading
 from pathlib import Path
 
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "librlt_b200.so"
+BINDING_PATH = LIB_PATH.with_name("_rlt_torch.so")
 
 F32, F16, BF16 = 0, 1, 2
 DTYPE_CODES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 
 OK = 0
-E_WORKSPACE = -4
 ERRORS = {
     -1: "unsupported dtype",
     -2: "unsupported head_dim",
@@ -170,17 +171,28 @@ def status_word(device: torch.device) -> torch.Tensor:
     return word
 
 
-_status_ptrs: dict[int, int] = {}
+_native = None
 
 
-def status_ptr(device: torch.device) -> int:
-    """Address of ``status_word(device)``, which lives as long as the process."""
-    address = _status_ptrs.get(device.index)
-    if address is None:
-        address = status_word(device).data_ptr()
-        if device.index is not None:
-            _status_ptrs[device.index] = address
-    return address
+def native():
+    """The torch extension (``csrc/binding.cpp``), loaded once; raise if it was
+    not built."""
+    global _native
+    if _native is None:
+        load()  # the library that it links
+        with _lock:
+            if _native is None:
+                if not BINDING_PATH.exists():
+                    raise RuntimeError(
+                        f"{BINDING_PATH} is missing: build it with "
+                        "`python -m vllm_rlt_b200._build` (there is no fallback implementation)")
+                spec = importlib.util.spec_from_file_location("_rlt_torch", BINDING_PATH)
+                module = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(module)
+                module.setup(
+                    lambda index: status_word(torch.device("cuda", index)).data_ptr(), check)
+                _native = module
+    return _native
 
 
 def read_status(device: torch.device, reset: bool = True) -> list[str]:
