@@ -29,7 +29,10 @@
 // here they are the 128-row operand and the activations the narrow one (16 to
 // 64 columns): a CTA streams 128 output features over its share of the input
 // features, a cluster of up to 8 CTAs shares a feature tile, and their partial
-// sums meet in distributed shared memory.
+// sums meet in distributed shared memory: each CTA reads the others' for the
+// rows that it finishes (stored there by the others with st.async instead, 64
+// rows took 9.4 us where reading takes 7.9). While the stream's previous kernel
+// still runs, the first weights are brought into L2.
 #include "proj_tc.cuh"
 
 namespace rlt {
@@ -402,10 +405,14 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
 
 // ---- few rows -----------------------------------------------------------------
 
-constexpr int kStreamThreads = 192;
+// Warps 0-3 move sums out of TMEM, 4 copies, 5 multiplies, and all finish rows:
+// twelve, so that at 64 rows and a cluster of six or more each has one row.
+constexpr int kStreamThreads = 384;
 constexpr int kStreamRows = 64;     // activation rows that stream_kernel takes
 constexpr int kStreamStages = 12;
 constexpr int kStreamFeatures = 128;
+
+constexpr int kStreamAhead = 16;  // blocks of weights brought into L2 ahead of time
 
 struct StreamParams {
   CUtensorMap map_x, map_w, map_up;
@@ -449,6 +456,20 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
     tc::fence_mbar_init();
   }
   if (warp == 5) tc::tmem_alloc(&tmem_slot, kTmemCols);
+  if (warp == 4 && tc::elect_one()) {
+    for (int kb = kb0; kb < min(kb1, kb0 + kStreamAhead); ++kb)
+#pragma unroll
+      for (int op = 0; op < kOps; ++op) {
+        const CUtensorMap* map = op ? &g.map_up : &g.map_w;
+        if (g.w_mn) {
+          tc::tma_prefetch_2d(map, n0, kb * kBlockK);
+          tc::tma_prefetch_2d(map, n0 + 64, kb * kBlockK);
+        } else {
+          tc::tma_prefetch_2d(map, kb * kBlockK, n0);
+        }
+      }
+  }
+  __syncwarp();
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
@@ -517,6 +538,18 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
     }
   }
   __syncwarp();
+  // What this thread's first row is finished with is on its way meanwhile.
+  const int n = n0 + lane * 4;
+  const int row_first = rank + warp * g.splits, row_step = kStreamThreads / 32 * g.splits;
+  const T* res = static_cast<const T*>(p.residual);
+  const T* bias = static_cast<const T*>(p.bias);
+  auto residual = [&](int row, float (&r)[4]) {
+    read4<T>(res != nullptr && n < p.outer && row < p.rows ? res + row * p.r_rs + n : nullptr,
+             g.vec, p.outer - n, r);
+  };
+  float b[4], r[4];
+  read4<T>(bias != nullptr && n < p.outer ? bias + n : nullptr, g.vec, p.outer - n, b);
+  residual(row_first, r);
   float* sums = reinterpret_cast<float*>(smem);  // [op][row][feature], where the stages were
   if (warp < 4) {
     ok = __all_sync(kFullMask, tc::mbar_wait(&acc_full, 0, kWaitLimit));
@@ -554,47 +587,50 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
     tc::tmem_dealloc(tmem, kTmemCols);
   }
   // Each CTA of the cluster finishes every splits-th row, adding in rank order:
-  // a warp per row, four neighbouring features per lane.
-  const int f0 = lane * 4;
-  const int n = n0 + f0;
-  if (n < p.outer) {
-    const T* res = static_cast<const T*>(p.residual);
-    const T* bias = static_cast<const T*>(p.bias);
-    float b[4];
-    read4<T>(bias != nullptr ? bias + n : bias, g.vec, p.outer - n, b);
-#pragma unroll 2
-    for (int row = rank + warp * g.splits; row < p.rows; row += kStreamThreads / 32 * g.splits) {
-      float r[4];
-      read4<T>(res != nullptr ? res + row * p.r_rs + n : res, g.vec, p.outer - n, r);
-      float y[kOps][4];
+  // a warp per row, four neighbouring features per lane. A warp that has read
+  // its last row lets the peers go before it turns the sums into outputs.
+  bool arrived = false;
+  for (int row = row_first; row < p.rows; row += row_step) {
+    float y[kOps][4];
 #pragma unroll
-      for (int op = 0; op < kOps; ++op) {
-        const float* mine = sums + (op * g.cols + row) * kStreamFeatures + f0;
-        float4 v[kMaxSplits];
+    for (int op = 0; op < kOps; ++op) {
+      const float* mine = sums + (op * g.cols + row) * kStreamFeatures + lane * 4;
+      float4 v[kMaxSplits];
 #pragma unroll
-        for (int s = 0; s < kMaxSplits; ++s)
-          if (s < g.splits) v[s] = g.splits > 1 ? tc::ld_peer4(tc::peer_smem(mine, s))
-                                                : *reinterpret_cast<const float4*>(mine);
-        float4 t = v[0];
+      for (int s = 0; s < kMaxSplits; ++s)
+        if (s < g.splits) v[s] = g.splits > 1 ? tc::ld_peer4(tc::peer_smem(mine, s))
+                                              : *reinterpret_cast<const float4*>(mine);
+      float4 t = v[0];
 #pragma unroll
-        for (int s = 1; s < kMaxSplits; ++s)
-          if (s < g.splits) {
-            t.x += v[s].x;
-            t.y += v[s].y;
-            t.z += v[s].z;
-            t.w += v[s].w;
-          }
-        y[op][0] = t.x;
-        y[op][1] = t.y;
-        y[op][2] = t.z;
-        y[op][3] = t.w;
-      }
-      finish4<T, kKind, kAct>(p, g.vec, row, n, y[0], y[kOps - 1], b, r);
+      for (int s = 1; s < kMaxSplits; ++s)
+        if (s < g.splits) {
+          t.x += v[s].x;
+          t.y += v[s].y;
+          t.z += v[s].z;
+          t.w += v[s].w;
+        }
+      y[op][0] = t.x;
+      y[op][1] = t.y;
+      y[op][2] = t.z;
+      y[op][3] = t.w;
     }
+    if (g.splits > 1 && row + row_step >= p.rows) {
+      float all = y[0][0] + y[0][1] + y[0][2] + y[0][3];
+      if (kOps == 2) all += y[kOps - 1][0] + y[kOps - 1][1] + y[kOps - 1][2] + y[kOps - 1][3];
+      __syncwarp();
+      tc::cluster_arrive(all);
+      arrived = true;
+    }
+    float next[4];
+    residual(row + row_step, next);
+    if (n < p.outer) finish4<T, kKind, kAct>(p, g.vec, row, n, y[0], y[kOps - 1], b, r);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] = next[e];
   }
+  __syncwarp();
   if (g.splits > 1) {
-    __syncwarp();
-    tc::cluster_sync();  // a peer may still be reading this CTA's sums
+    if (!arrived) tc::cluster_arrive(0.f);
+    tc::cluster_wait();  // a peer may still be reading this CTA's sums
   }
 }
 
@@ -695,15 +731,41 @@ int run_stream(Kind kind, const Problem& p, int32_t dtype, int ctas, cudaStream_
   g.stage_bytes = ops * kStreamFeatures * kBlockK * 2 + g.cols * 128;
   const int tiles = ceil_div(p.outer, kStreamFeatures);
   const int kblocks = ceil_div(p.inner, kBlockK);
-  // a cluster wide enough that the CTAs fill the SMs about twice
-  g.splits = 1;
-  while (g.splits < kMaxSplits && g.splits < kblocks && tiles * (g.splits + 1) <= 2 * ctas) ++g.splits;
-  const int share = ceil_div(kblocks, g.splits);
-  // two CTAs fit an SM, so that a cluster finds room whatever the number of
-  // SMs its part of the die has
-  g.stages = 110 * 1024 / g.stage_bytes;
+  // CTAs per tile and shared memory per CTA: the least weights per SM, where
+  // either one CTA of 200 KB runs on an SM (its clusters then have to fit the
+  // die's parts) or two of 110 KB. The partial sums of many rows cost more to
+  // exchange in wide clusters: at 64 rows 3 x 200 KB takes 14.1 us for the gated
+  // product and 6 x 110 KB 15.9, while one row takes 11.6 and 10.9; 64 rows of
+  // 2048 x 2048 take 6.9 us with 6 x 200 KB and 7.6 with 8 x 110 KB.
+  const bool many = p.rows > 16;
+  constexpr int kBig = 200 * 1024, kSmall = 110 * 1024;
+  double least = 1e300;
+  int budget = kSmall;
+  for (int s = 1; s <= kMaxSplits && s <= kblocks; ++s) {
+    for (int big = 0; big < 2; ++big) {
+      constexpr auto kernel = stream_kernel<__half, kLinear, RLT_ACT_NONE>;
+      int waves;
+      if (big) {
+        if (s > 6) continue;
+        const int at_once = s == 1 ? ctas : resident_clusters<kernel>(s, kStreamThreads, kBig);
+        if (s > 1 && tiles > at_once) continue;
+        waves = ceil_div(tiles, at_once);
+      } else {
+        if (s > 1 && tiles * s > 2 * ctas) continue;
+        waves = ceil_div(tiles * s, ctas);
+      }
+      const double cost = static_cast<double>(waves) / s * (big == many ? 1.0 : 1.5);
+      if (cost < least * (many ? 0.999 : 1.001)) {
+        least = cost;
+        g.splits = s;
+        budget = big ? kBig : kSmall;
+      }
+    }
+  }
+  const int per_cta = ceil_div(kblocks, g.splits);
+  g.stages = budget / g.stage_bytes;
   if (g.stages > kStreamStages) g.stages = kStreamStages;
-  if (g.stages > share) g.stages = share;
+  if (g.stages > per_cta) g.stages = per_cta;
   const int sums = ops * g.cols * kStreamFeatures * 4;  // partial sums lie where the stages were
   while (g.stages * g.stage_bytes < sums) ++g.stages;
   bool ok = encode2d(&g.map_x, dtype, p.x, p.inner, p.rows, p.x_rs, g.cols);

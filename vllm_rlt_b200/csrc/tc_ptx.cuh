@@ -160,7 +160,16 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, u
       : "memory");
 }
 
-// The same from either CTA of a pair into its own shared memory, completing on
+// Bring a tile into L2 only. Nothing reads it: a later write to the same memory
+// is what a later load sees.
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int c0, int c1) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(c0), "r"(c1)
+               : "memory");
+}
+
+// tma_load_2d from either CTA of a pair into its own shared memory, completing on
 // the barrier at this offset in the pair's first CTA (bit 24 of a shared
 // address tells the two CTAs apart).
 __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint64_t* bar,
@@ -284,6 +293,15 @@ __device__ __forceinline__ void mbar_arrive_at(uint64_t* bar, uint32_t rank) {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
                    : "memory");
+}
+
+// The two halves of cluster_sync. The arrival follows from `after`: what that
+// was computed from has been read.
+__device__ __forceinline__ void cluster_arrive(float after) {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::"f"(after) : "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
