@@ -206,7 +206,9 @@ int resident_clusters(int size, int threads, int smem) {
   if (cudaGetDevice(&dev) != cudaSuccess) return 1;
   if (dev >= 0 && dev < 64)
     if (const int n = known[dev][size].load()) return n;
-  if (allow_smem<kKernel>(smem) != cudaSuccess) return 1;
+  if (cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBudget) !=
+      cudaSuccess)
+    return 1;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(size);
   cfg.blockDim = dim3(threads);

@@ -18,11 +18,13 @@
 // NaN. Any NaN that comes out is recomputed by fp32 multiply-adds from the
 // operands, so infinities and NaN end up as they would there.
 //
-// A CTA (16 warps) takes a tile of 128 rows by 128 weight rows over its share of
+// A CTA (20 warps) takes a tile of 128 rows by 128 weight rows over its share of
 // the input features; a cluster of up to 8 CTAs shares a tile when there are few.
-// Warp 14 copies slices of 32 input features (fp32, 128 bytes) by TMA, warps
-// 0-13 split them into parts in shared memory, warp 15 issues the products, and
-// warps 0-7 gather the sums between slices. Per slice of 128 x 128 shared memory moves 32 KB
+// Warp 16 copies slices of 32 input features (fp32, 128 bytes) by TMA, warps
+// 8-15 split them into parts in shared memory (two groups that take every other
+// slice, so that one's waits and fences lie under the other's work), warp 17
+// issues the products, and warps 0-7 gather the sums and finish the outputs. Per
+// slice of 128 x 128 shared memory moves 32 KB
 // in, 80 KB through the split and 96 KB into the tensor core, about 1660
 // cycles against 768 of arithmetic: that traffic bounds the kernel.
 #include "proj_tc.cuh"
@@ -31,7 +33,7 @@ namespace rlt {
 namespace proj {
 namespace {
 
-constexpr int kSplitThreads = 16 * 32;
+constexpr int kSplitThreads = 20 * 32;
 constexpr int kSlice = 32;                   // input features per slice
 constexpr int kTile = 128;                   // rows, and weight rows, of a tile
 constexpr int kRawBytes = kTile * 128;       // one operand's slice as it arrives
@@ -40,8 +42,12 @@ constexpr int kRawStages = 3, kPartStages = 2;
 constexpr int kRawStage = 2 * kRawBytes, kPartStage = 6 * kPartBytes;
 constexpr int kSplitSmem = kRawStages * kRawStage + kPartStages * kPartStage + 1024;
 constexpr int kSumSlices = 512 / kSlice;     // slices accumulated in TMEM at a time
-constexpr int kConvertWarps = 14, kCopyWarp = 14, kIssueWarp = 15;
-constexpr int kGroupWarps = kConvertWarps / 2;  // even slices, odd slices
+constexpr int kGatherWarps = 8, kGroupWarps = 4, kCopyWarp = 16, kIssueWarp = 17;
+// Registers per thread: at launch, and as the warpgroups share them out.
+constexpr int kSplitLaunchRegs = 96, kGatherRegs = 136, kConvertRegs = 80, kIssueRegs = 40;
+static_assert(256 * (kGatherRegs + kConvertRegs) + 128 * kIssueRegs <=
+                  kSplitThreads * kSplitLaunchRegs,
+              "the increase draws on what the launch allocated");
 
 struct SplitParams {
   CUtensorMap map_x, map_w, map_up;
@@ -84,8 +90,16 @@ __device__ __forceinline__ uint64_t smem_desc_sw64(uint32_t addr) {
   return d;
 }
 
+// A wait ran out: let copies in flight land before the memory goes.
+__device__ __forceinline__ void drain(volatile int* aborted) {
+  *aborted = 1;
+  const long long start = clock64();
+  while (clock64() - start < 4000000LL) {
+  }
+}
+
 // x[row] . w[n] in fp32 multiply-adds.
-__device__ __noinline__ float plain_dot(const Problem& p, const float* w, int row, int n) {
+__device__ __forceinline__ float plain_dot(const Problem& p, const float* w, int row, int n) {
   const float* x = static_cast<const float*>(p.x) + row * p.x_rs;
   w += n * p.w_ns;
   float y = 0.f;
@@ -143,92 +157,159 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   tc::pdl_wait();
   const uint32_t tmem = tmem_slot;
   bool ok = true;
-  float v[64];  // warps 0-7: this thread's row, half of the columns
 
-  if (warp == kCopyWarp) {
-    const uint32_t bytes = kRawBytes + g.box_m * 128;
-    Ring at;
-    for (int i = 0; i < count; ++i, at.next(kRawStages)) {
-      if (!__all_sync(kFullMask, tc::mbar_wait(&raw_empty[at.slot], at.parity ^ 1, kWaitLimit))) {
-        ok = false;
-        break;
-      }
-      if (tc::elect_one()) {
-        uint64_t* bar = &raw_full[at.slot];
-        uint8_t* x = raw + at.slot * kRawStage;
-        uint8_t* w = x + kRawBytes;
-        const int k0 = (first + i) * kSlice;
-        tc::mbar_expect_tx(bar, bytes);
-        tc::tma_load_2d(x, &g.map_x, bar, k0, m0);
-        if (g.w_mn) {  // boxes of 32 output features by 32 input features
-#pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            const bool second = kKind == kGated && b >= 2;
-            tc::tma_load_2d(w + b * 4096, second ? &g.map_up : &g.map_w, bar,
-                            n0 + b * 32 - (second ? kSet : 0), k0);
-          }
-        } else {
-          tc::tma_load_2d(w, &g.map_w, bar, k0, n0);
-          if (kKind == kGated) tc::tma_load_2d(w + kRawBytes / 2, &g.map_up, bar, k0, n0);
+  if (warp >= kCopyWarp) {
+    tc::setmaxnreg_dec<kIssueRegs>();
+    if (warp == kCopyWarp) {
+      const uint32_t bytes = kRawBytes + g.box_m * 128;
+      Ring at;
+      for (int i = 0; i < count; ++i, at.next(kRawStages)) {
+        if (!__all_sync(kFullMask, tc::mbar_wait(&raw_empty[at.slot], at.parity ^ 1, kWaitLimit))) {
+          ok = false;
+          break;
         }
+        if (tc::elect_one()) {
+          uint64_t* bar = &raw_full[at.slot];
+          uint8_t* x = raw + at.slot * kRawStage;
+          uint8_t* w = x + kRawBytes;
+          const int k0 = (first + i) * kSlice;
+          tc::mbar_expect_tx(bar, bytes);
+          tc::tma_load_2d(x, &g.map_x, bar, k0, m0);
+          if (g.w_mn) {  // boxes of 32 output features by 32 input features
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+              const bool second = kKind == kGated && b >= 2;
+              tc::tma_load_2d(w + b * 4096, second ? &g.map_up : &g.map_w, bar,
+                              n0 + b * 32 - (second ? kSet : 0), k0);
+            }
+          } else {
+            tc::tma_load_2d(w, &g.map_w, bar, k0, n0);
+            if (kKind == kGated) tc::tma_load_2d(w + kRawBytes / 2, &g.map_up, bar, k0, n0);
+          }
+        }
+        __syncwarp();
       }
-      __syncwarp();
-    }
-  } else if (warp == kIssueWarp) {
-    const uint32_t idesc = tc::idesc_f16(1, kTile, kTile, g.w_mn);
-    const uint64_t x_desc = smem_desc_sw64(tc::smem_u32(parts));
-    const uint64_t w_desc = g.w_mn ? tc::smem_desc_sw128(tc::smem_u32(parts) + 3 * kPartBytes, 4096, 1024)
-                                   : smem_desc_sw64(tc::smem_u32(parts) + 3 * kPartBytes);
-    const uint32_t x_hi = static_cast<uint32_t>(x_desc >> 32);
-    const uint32_t w_hi = static_cast<uint32_t>(w_desc >> 32);
-    const uint32_t kstep_w = (g.w_mn ? 2048 : 32) >> 4;
-    Ring at, acc;
-    for (int i = 0; ok && i < count; acc.next(2)) {
-      if (!__all_sync(kFullMask, tc::mbar_poll(&acc_empty[acc.slot], acc.parity ^ 1, kWaitLimit))) {
-        ok = false;
-        break;
-      }
-      tc::tc_fence_after();
-      const uint32_t d = tmem + acc.slot * 256;
-      const int end = min(i + kSumSlices, count);
-      for (uint32_t more = 0; i < end; ++i, at.next(kPartStages)) {
-        if (!__all_sync(kFullMask, tc::mbar_poll(&part_full[at.slot], at.parity, kWaitLimit))) {
+    } else if (warp == kIssueWarp) {
+      const uint32_t idesc = tc::idesc_f16(1, kTile, kTile, g.w_mn);
+      const uint64_t x_desc = smem_desc_sw64(tc::smem_u32(parts));
+      const uint64_t w_desc =
+          g.w_mn ? tc::smem_desc_sw128(tc::smem_u32(parts) + 3 * kPartBytes, 4096, 1024)
+                 : smem_desc_sw64(tc::smem_u32(parts) + 3 * kPartBytes);
+      const uint32_t x_hi = static_cast<uint32_t>(x_desc >> 32);
+      const uint32_t w_hi = static_cast<uint32_t>(w_desc >> 32);
+      const uint32_t kstep_w = (g.w_mn ? 2048 : 32) >> 4;
+      Ring at, acc;
+      for (int i = 0; ok && i < count; acc.next(2)) {
+        if (!__all_sync(kFullMask,
+                        tc::mbar_poll(&acc_empty[acc.slot], acc.parity ^ 1, kWaitLimit))) {
           ok = false;
           break;
         }
         tc::tc_fence_after();
-        if (tc::elect_one()) {
-          const uint32_t x_lo = static_cast<uint32_t>(x_desc) + at.slot * (kPartStage >> 4);
-          const uint32_t w_lo = static_cast<uint32_t>(w_desc) + at.slot * (kPartStage >> 4);
-          auto product = [&](uint32_t acc_at, int xp, int wp, int ks, uint32_t accumulate) {
-            tc::mma_f16_ss(acc_at, tc::desc64(x_lo + xp * (kPartBytes >> 4) + ks * 2, x_hi),
-                           tc::desc64(w_lo + wp * (kPartBytes >> 4) + ks * kstep_w, w_hi), idesc,
-                           accumulate);
-          };
-#pragma unroll
-          for (int ks = 0; ks < kSlice / 16; ++ks) {
-            const uint32_t go = ks > 0 ? 1 : more;
-            product(d, 0, 0, ks, go);
-            product(d + kTile, 0, 2, ks, go);
-            product(d + kTile, 2, 0, ks, 1);
-            product(d + kTile, 1, 1, ks, 1);
-            product(d + kTile, 0, 1, ks, 1);
-            product(d + kTile, 1, 0, ks, 1);
+        const uint32_t d = tmem + acc.slot * 256;
+        const int end = min(i + kSumSlices, count);
+        for (uint32_t more = 0; i < end; ++i, at.next(kPartStages)) {
+          if (!__all_sync(kFullMask, tc::mbar_poll(&part_full[at.slot], at.parity, kWaitLimit))) {
+            ok = false;
+            break;
           }
-          tc::mma_commit(&part_empty[at.slot]);
-          if (i == end - 1) tc::mma_commit(&acc_full[acc.slot]);
+          tc::tc_fence_after();
+          if (tc::elect_one()) {
+            const uint32_t x_lo = static_cast<uint32_t>(x_desc) + at.slot * (kPartStage >> 4);
+            const uint32_t w_lo = static_cast<uint32_t>(w_desc) + at.slot * (kPartStage >> 4);
+            auto product = [&](uint32_t acc_at, int xp, int wp, int ks, uint32_t accumulate) {
+              tc::mma_f16_ss(acc_at, tc::desc64(x_lo + xp * (kPartBytes >> 4) + ks * 2, x_hi),
+                             tc::desc64(w_lo + wp * (kPartBytes >> 4) + ks * kstep_w, w_hi), idesc,
+                             accumulate);
+            };
+#pragma unroll
+            for (int ks = 0; ks < kSlice / 16; ++ks) {
+              const uint32_t go = ks > 0 ? 1 : more;
+              product(d, 0, 0, ks, go);
+              product(d + kTile, 0, 2, ks, go);
+              product(d + kTile, 2, 0, ks, 1);
+              product(d + kTile, 1, 1, ks, 1);
+              product(d + kTile, 0, 1, ks, 1);
+              product(d + kTile, 1, 0, ks, 1);
+            }
+            tc::mma_commit(&part_empty[at.slot]);
+            if (i == end - 1) tc::mma_commit(&acc_full[acc.slot]);
+          }
+          more = 1;
+          __syncwarp();
         }
-        more = 1;
-        __syncwarp();
       }
     }
+    if (!ok) drain(&aborted);
+    __syncwarp();
+    if (kKind != kVocab && g.splits > 1) {
+      tc::cluster_sync();
+      tc::cluster_sync();
+    }
+  } else if (warp >= kGatherWarps) {
+    tc::setmaxnreg_dec<kConvertRegs>();
+    // A warp takes one 32-byte column of the slice's 128-byte lines: 8 elements
+    // of 32 lines at a time. Neighbouring lanes have neighbouring lines (rows, or
+    // input features of an MN-major slice), which keeps reads and writes free of
+    // bank conflicts, and every address is a constant away from the lane's first.
+    const int group = (warp - kGatherWarps) / kGroupWarps, c = warp % kGroupWarps;
+    const uint32_t from = lane * 128 + (((2 * c) ^ (lane & 7)) << 4);
+    const uint32_t to_k = lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4);
+    const uint32_t to_mn = lane * 128 + ((c ^ (lane & 7)) << 4);
+    auto convert = [&](const uint8_t* line, uint32_t at, uint8_t* to) {
+      uint4 part[3];
+      split8(*reinterpret_cast<const float4*>(line + at),
+             *reinterpret_cast<const float4*>(line + (at ^ 16)), part);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4*>(to + k * kPartBytes) = part[k];
+    };
+    Ring at;
+    if (group) at.next(kRawStages);
+    uint32_t parity = 1;
+    for (int i = group; i < count; i += 2) {
+      ok = __all_sync(kFullMask, tc::mbar_wait(&raw_full[at.slot], at.parity, kWaitLimit) &&
+                                     tc::mbar_wait(&part_empty[group], parity, kWaitLimit));
+      if (!ok) break;
+      const uint8_t* src = raw + at.slot * kRawStage;
+      uint8_t* dst = parts + group * kPartStage;
+      if (g.w_mn) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          convert(src + kRawBytes + j * 4096, from,
+                  dst + 3 * kPartBytes + (j >> 1) * 4096 + (to_mn ^ ((j & 1) << 6)));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          convert(src + kRawBytes + j * 4096, from, dst + 3 * kPartBytes + j * 2048 + to_k);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j * 32 + lane < g.box_m) convert(src + j * 4096, from, dst + j * 2048 + to_k);
+      tc::fence_proxy_async_smem();  // the parts are read by the tensor core
+      __syncwarp();
+      if (lane == 0) {
+        tc::mbar_arrive(&part_full[group]);
+        tc::mbar_arrive(&raw_empty[at.slot]);
+      }
+      parity ^= 1;
+      at.next(kRawStages);
+      at.next(kRawStages);
+    }
+    if (!ok) drain(&aborted);
+    __syncwarp();
+    if (kKind != kVocab && g.splits > 1) {
+      tc::cluster_sync();
+      tc::cluster_sync();
+    }
   } else {
-    // The next group's sums into v (warps 0-7).
-    const uint32_t taddr = tmem + (static_cast<uint32_t>(warp & 3) << 21) + (warp >> 2) * 64;
+    tc::setmaxnreg_inc<kGatherRegs>();
+    float v[64];  // this thread's row, half of the columns
+    const int half = warp >> 2;
+    const uint32_t taddr = tmem + (static_cast<uint32_t>(warp & 3) << 21) + half * 64;
     Ring acc;
-    auto gather = [&](bool first_group) {
+    for (int i = 0; i < count; i += kSumSlices, acc.next(2)) {
       ok = __all_sync(kFullMask, tc::mbar_wait(&acc_full[acc.slot], acc.parity, kWaitLimit));
-      if (!ok) return;
+      if (!ok) break;
       tc::tc_fence_after();
 #pragma unroll
       for (int c = 0; c < 64; c += 16) {
@@ -240,93 +321,28 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const float t = __uint_as_float(big[j]) + __uint_as_float(small[j]);
-          v[c + j] = first_group ? t : v[c + j] + t;
+          v[c + j] = i == 0 ? t : v[c + j] + t;
         }
       }
       tc::tc_fence_before();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&acc_empty[acc.slot]);
-      acc.next(2);
-    };
-    // A warp's unit is 32 lines of 8 elements. Neighbouring lanes take
-    // neighbouring lines (rows, or input features of an MN-major slice), which
-    // keeps reads and writes free of bank conflicts.
-    const int x_units = (g.box_m + 31) / 32 * 4, units = x_units + kTile / 8;
-    // Two groups of warps take every other slice, each with a part stage of its
-    // own, so that one group's waits and fences lie under the other's work.
-    const int group = warp & 1, member = warp >> 1;
-    Ring at_raw;
-    if (group) at_raw.next(kRawStages);
-    uint32_t part_parity = 1;
-    int gathered = 0;  // slices whose sums are in v
-    for (int i = group; i < count; i += 2) {
-      ok = __all_sync(kFullMask,
-                      tc::mbar_wait(&raw_full[at_raw.slot], at_raw.parity, kWaitLimit) &&
-                          tc::mbar_wait(&part_empty[group], part_parity, kWaitLimit));
-      if (!ok) break;
-      const uint8_t* src = raw + at_raw.slot * kRawStage;
-      uint8_t* dst = parts + group * kPartStage;
-      for (int u = member; u < units; u += kGroupWarps) {
-        const bool of_x = u < x_units;
-        const int q = of_x ? u : u - x_units;
-        const uint8_t* r;  // the line's 128 bytes
-        uint8_t* t;
-        int line = lane, c = q & 3;
-        if (of_x || !g.w_mn) {
-          line += q / 4 * 32;
-          r = src + (of_x ? 0 : kRawBytes) + line * 128;
-          t = dst + (of_x ? 0 : 3 * kPartBytes) + line * 64 + ((c ^ ((line >> 1) & 3)) << 4);
-        } else {
-          r = src + kRawBytes + q / 4 * 4096 + line * 128;
-          t = dst + 3 * kPartBytes + q / 8 * 4096 + line * 128 + (((q & 7) ^ (line & 7)) << 4);
-        }
-        if (!of_x || line < g.box_m) {
-          uint4 part[3];
-          split8(*reinterpret_cast<const float4*>(r + (((2 * c) ^ (line & 7)) << 4)),
-                 *reinterpret_cast<const float4*>(r + (((2 * c + 1) ^ (line & 7)) << 4)), part);
-#pragma unroll
-          for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4*>(t + k * kPartBytes) = part[k];
-        }
-      }
-      tc::fence_proxy_async_smem();  // the parts are read by the tensor core
-      __syncwarp();
-      if (lane == 0) {
-        tc::mbar_arrive(&part_full[group]);
-        tc::mbar_arrive(&raw_empty[at_raw.slot]);
-      }
-      part_parity ^= 1;
-      at_raw.next(kRawStages);
-      at_raw.next(kRawStages);
-      // these sums' last products were issued slices ago
-      if (warp < 8 && i >= gathered + kSumSlices + 2) {
-        gather(gathered == 0);
-        if (!ok) break;
-        gathered += kSumSlices;
-      }
     }
-    for (; ok && warp < 8 && gathered < count; gathered += kSumSlices) gather(gathered == 0);
-  }
-  if (!ok) {  // a wait ran out: let copies in flight land before the memory goes
-    aborted = 1;
-    const long long start = clock64();
-    while (clock64() - start < 4000000LL) {
-    }
-  }
-  __syncwarp();
-
-  const int half = warp >> 2;
-  if constexpr (kKind == kVocab) {
-    if (warp < 8) {
+    if (!ok) drain(&aborted);
+    __syncwarp();
+    if constexpr (kKind == kVocab) {
       const int row = m0 + (warp & 3) * 32 + lane, at = n0 + half * 64;
       const int cols = min(64, p.outer - at);
       bool odd = false;
 #pragma unroll
       for (int j = 0; j < 64; ++j) odd = odd || (j < cols && v[j] != v[j]);
       if (odd && row < p.rows) {
+        for (int i = 0; i < cols; ++i) {
+          const float y = plain_dot(p, static_cast<const float*>(p.w), row, at + i);
 #pragma unroll
-        for (int j = 0; j < 64; ++j)
-          if (j < cols && v[j] != v[j])
-            v[j] = plain_dot(p, static_cast<const float*>(p.w), row, at + j);
+          for (int j = 0; j < 64; ++j)
+            if (j == i && v[j] != v[j]) v[j] = y;
+        }
       }
       __syncwarp();
       const int64_t want = p.tokens != nullptr && row < p.rows ? p.tokens[row] : -1;
@@ -335,79 +351,85 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
         *reinterpret_cast<float4*>(
             &p.parts[static_cast<int64_t>(row) * p.tiles + tile / g.row_tiles * 2 + half]) =
             make_float4(part.most, part.sum, __int_as_float(part.at), part.chosen);
-    }
-  } else {
-    // every role is done with the stages: the sums take their place, rows of
-    // 128 columns (gate then up) in 16-byte units swizzled by row
-    __syncthreads();
-    if (warp < 8) {
-      const int r = (warp & 3) * 32 + lane;
+    } else {
+      // Every product is done, so the stages are free: the sums take their place,
+      // rows of 128 columns (gate then up) in 16-byte units swizzled by row.
+      const int r0 = (warp & 3) * 32 + lane;
 #pragma unroll
       for (int c = 0; c < 16; ++c)
-        *reinterpret_cast<float4*>(smem + r * 512 + (((half * 16 + c) ^ (r & 7)) << 4)) =
+        *reinterpret_cast<float4*>(smem + r0 * 512 + (((half * 16 + c) ^ (r0 & 7)) << 4)) =
             make_float4(v[c * 4], v[c * 4 + 1], v[c * 4 + 2], v[c * 4 + 3]);
-    }
-    if (g.splits > 1)
-      tc::cluster_sync();
-    else
-      __syncthreads();
-    // Each CTA of the cluster finishes every splits-th row, adding in rank order.
-    constexpr int kLanes = kSet / 4;  // lanes per row, four features each
-    const int c = lane % kLanes, n = n0 + c * 4;
-    const int rows = min(kTile, p.rows - m0);
-    if (n < p.outer) {
+      // Each CTA of the cluster finishes every splits-th row, adding in rank order.
+      constexpr int kLanes = kSet / 4;  // lanes per row, four features each
+      const int c = lane % kLanes, n = n0 + c * 4;
+      const int rows = min(kTile, p.rows - m0);
+      const int row_first = rank + (warp * (32 / kLanes) + lane / kLanes) * g.splits;
+      const int row_step = kGatherWarps * (32 / kLanes) * g.splits;
       const float* bias_at = static_cast<const float*>(p.bias);
       const float* res_at = static_cast<const float*>(p.residual);
-      float bias[4];
-      read4<float>(bias_at != nullptr ? bias_at + n : nullptr, g.vec, p.outer - n, bias);
-      constexpr int kRowsPerPass = kSplitThreads / kLanes;
-#pragma unroll 2
-      for (int r = rank + (warp * (32 / kLanes) + lane / kLanes) * g.splits; r < rows;
-           r += kRowsPerPass * g.splits) {
-        float add[4];
-        read4<float>(res_at != nullptr ? res_at + (m0 + r) * p.r_rs + n : nullptr, g.vec,
-                     p.outer - n, add);
-        float y[2][4];
+      auto residual = [&](int r, float (&add)[4]) {
+        read4<float>(res_at != nullptr && n < p.outer && r < rows ? res_at + (m0 + r) * p.r_rs + n
+                                                                  : nullptr,
+                     g.vec, p.outer - n, add);
+      };
+      float bias[4], add[4];
+      read4<float>(bias_at != nullptr && n < p.outer ? bias_at + n : nullptr, g.vec, p.outer - n,
+                   bias);
+      residual(row_first, add);
+      if (g.splits > 1)
+        tc::cluster_sync();
+      else
+        asm volatile("bar.sync 1, %0;" ::"n"(kGatherWarps * 32) : "memory");
+      if (n < p.outer) {
+        for (int r = row_first; r < rows; r += row_step) {
+          float y[2][4];
 #pragma unroll
-        for (int op = 0; op < (kKind == kGated ? 2 : 1); ++op) {
-          const uint8_t* at = smem + r * 512 + (((op * 16 + c) ^ (r & 7)) << 4);
-          float4 t[kMaxSplits];
+          for (int op = 0; op < (kKind == kGated ? 2 : 1); ++op) {
+            const uint8_t* at = smem + r * 512 + (((op * 16 + c) ^ (r & 7)) << 4);
+            float4 t[kMaxSplits];
 #pragma unroll
-          for (int s = 0; s < kMaxSplits; ++s)
-            if (s < g.splits)
-              t[s] = g.splits > 1 ? tc::ld_peer4(tc::peer_smem(at, s))
-                                  : *reinterpret_cast<const float4*>(at);
+            for (int s = 0; s < kMaxSplits; ++s)
+              if (s < g.splits)
+                t[s] = g.splits > 1 ? tc::ld_peer4(tc::peer_smem(at, s))
+                                    : *reinterpret_cast<const float4*>(at);
 #pragma unroll
-          for (int s = 1; s < kMaxSplits; ++s)
-            if (s < g.splits) {
-              t[0].x += t[s].x;
-              t[0].y += t[s].y;
-              t[0].z += t[s].z;
-              t[0].w += t[s].w;
+            for (int s = 1; s < kMaxSplits; ++s)
+              if (s < g.splits) {
+                t[0].x += t[s].x;
+                t[0].y += t[s].y;
+                t[0].z += t[s].z;
+                t[0].w += t[s].w;
+              }
+            y[op][0] = t[0].x;
+            y[op][1] = t[0].y;
+            y[op][2] = t[0].z;
+            y[op][3] = t[0].w;
+            const float any = y[op][0] + y[op][1] + y[op][2] + y[op][3];
+            if (any != any) {
+              const float* w = static_cast<const float*>(op == 0 ? p.w : p.w_up);
+              for (int i = 0; i < 4 && n + i < p.outer; ++i) {
+                const float plain = plain_dot(p, w, m0 + r, n + i);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (e == i && y[op][e] != y[op][e]) y[op][e] = plain;
+              }
             }
-          y[op][0] = t[0].x;
-          y[op][1] = t[0].y;
-          y[op][2] = t[0].z;
-          y[op][3] = t[0].w;
-          const float* w = static_cast<const float*>(op == 0 ? p.w : p.w_up);
-          const float any = y[op][0] + y[op][1] + y[op][2] + y[op][3];
-          if (any != any) {
-            for (int e = 0; e < 4; ++e)
-              if (y[op][e] != y[op][e] && n + e < p.outer)
-                y[op][e] = plain_dot(p, w, m0 + r, n + e);
           }
+          float next[4];
+          residual(r + row_step, next);
+          finish4<float, kKind, kAct>(p, g.vec, m0 + r, n, y[0], y[kKind == kGated ? 1 : 0], bias,
+                                      add);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) add[e] = next[e];
         }
-        finish4<float, kKind, kAct>(p, g.vec, m0 + r, n, y[0], y[kKind == kGated ? 1 : 0], bias,
-                                    add);
       }
+      __syncwarp();
+      if (g.splits > 1) tc::cluster_sync();  // a peer may still be reading this CTA's sums
     }
   }
   __syncwarp();
   tc::tc_fence_before();
-  if (g.splits > 1)
-    tc::cluster_sync();  // a peer may still be reading this CTA's sums
-  else
-    __syncthreads();
+  __syncthreads();
   if (aborted && threadIdx.x == 0) raise_status(p.status, kStatusTimeout);
   if (warp == kIssueWarp) {
     tc::tc_fence_after();
@@ -418,7 +440,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
 template <typename T, Kind kKind, int kAct>
 int launch(const SplitParams& g, int ctas, cudaStream_t stream) {
   constexpr auto kernel = split_kernel<T, kKind, kAct>;
-  if (const cudaError_t e = allow_smem<kernel>(kSplitSmem)) return static_cast<int>(e);
+  if (const cudaError_t e = allow_smem<kernel>(kSplitSmem, kSplitLaunchRegs)) return static_cast<int>(e);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(ctas));
   cfg.blockDim = dim3(kSplitThreads);
