@@ -405,3 +405,100 @@ def test_feed_forward_block_and_head(rows, layout):
     at = tokens[:, None]
     assert_within(logprobs, lp.gather(1, at)[:, 0], bound.gather(1, at)[:, 0])
     assert torch.equal(rb.token_logprobs(hidden, head, tokens), logprobs)
+
+
+# ------------------------------------------------- together on one device, extremes
+
+
+@pytest.mark.parametrize("rows", [3, 64])
+def test_types_on_two_streams_at_once(rows):
+    """fp32 and 16-bit calls split their sums over clusters of CTAs that wait for
+    one another; both kinds run at once without holding each other up."""
+    made = [calls(torch.bfloat16, rows)[1], calls(torch.float32, rows)[1]]
+    want = [call() for call in made]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(40):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(made[i]())
+    torch.cuda.synchronize()
+    assert _lib.read_status(torch.device("cuda", 0)) == []
+    for i in range(2):
+        for result in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(result, want[i]))
+
+
+FIRST_CALL_CAPTURED = """
+import torch, vllm_rlt_b200 as rb
+x = torch.randn(%d, 128, device="cuda").to(torch.%s)
+w = torch.randn(256, 128, device="cuda").to(torch.%s)
+torch.cuda.synchronize()
+rb._lib.status_word(x.device)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y, h, t = rb.linear(x, w), rb.gated_linear(x, w), rb.greedy_tokens(x, w)
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(y, rb.linear(x, w)) and torch.equal(h, rb.gated_linear(x, w))
+assert all(torch.equal(a, b) for a, b in zip(t, rb.greedy_tokens(x, w)))
+"""
+
+
+@pytest.mark.parametrize("rows,dtype", [(5, "bfloat16"), (300, "bfloat16"), (5, "float32")])
+def test_the_first_call_may_be_captured(rows, dtype):
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    subprocess.run([sys.executable, "-c", FIRST_CALL_CAPTURED % (rows, dtype, dtype)], check=True,
+                   cwd=Path(__file__).resolve().parents[1], timeout=300)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("inner,outer", [(40000, 3), (20011, 70)])
+def test_long_sums(inner, outer, dtype):
+    g = generator(61)
+    for rows in (2, 90):
+        x = normal(g, rows, inner, dtype=dtype)
+        w = normal(g, outer, inner, std=0.05, dtype=dtype)
+        assert_within(rb.linear(x, w), *po.linear(x, w))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_offsets_beyond_32_bits(dtype):
+    """Rows of x, residual and out lie 2^31 and more elements apart."""
+    g = generator(62)
+    gap = 2 ** 30 + 16
+    room = torch.zeros(3 * gap + 4096, device="cuda", dtype=dtype)
+    rows = [room.as_strided((4, n), (gap, 1), at) for n, at in ((128, 0), (64, 1024), (64, 2048))]
+    x, residual, out = rows
+    x.copy_(normal(g, 4, 128))
+    residual.copy_(normal(g, 4, 64))
+    w = normal(g, 64, 128, std=0.05, dtype=dtype)
+    rb.linear(x, w, residual=residual, out=out)
+    assert_within(out, *po.linear(x, w, residual=residual))
+    head = room.as_strided((4, 128), (gap, 1), 3072)  # weights far apart as well
+    head.copy_(normal(g, 4, 128))
+    assert_within(rb.linear(x, head), *po.linear(x, head))
+
+
+def test_a_row_of_infinities_and_not_numbers_in_single_precision():
+    """fp32 splits its operands; what the split cannot carry is recomputed."""
+    g = generator(63)
+    for rows in (4, 150):
+        x, w = normal(g, rows, 96), normal(g, 130, 96, std=0.05)
+        x[0, 3], x[1, 4], x[2] = float("inf"), -float("inf"), float("nan")
+        x[3, 0], x[3, 1] = float("inf"), float("nan")
+        w[7, 3], w[9, 4], w[11] = 0.0, 0.5, float("inf")
+        got = rb.linear(x, w)
+        want = (x.double()[:, None] * w.double()[None]).sum(-1)
+        assert torch.equal(got.isnan(), want.isnan())
+        inf = want.isinf()
+        assert torch.equal(got[inf].double(), want[inf])
+        fine = want.isfinite()
+        assert fine.any() or rows == 4
+        close = po.linear(torch.nan_to_num(x, 0, 0, 0), torch.nan_to_num(w, 0, 0, 0))
+        off = (got.double() - close[0]).abs() - close[1]
+        assert bool((off[fine] <= 0).all())

@@ -14,6 +14,10 @@ namespace proj {
 namespace {
 
 constexpr long long kWaitLimit = 100000000LL;  // cycles (~50 ms)
+// For a wait that covers `blocks` blocks of input features.
+__device__ __forceinline__ long long whole_sum_limit(int blocks) {
+  return kWaitLimit + blocks * 20000LL;
+}
 constexpr int kMaxSplits = 8;                  // CTAs of a cluster (the portable limit)
 constexpr int kSmemBudget = 224 * 1024;        // dynamic shared memory of a CTA
 

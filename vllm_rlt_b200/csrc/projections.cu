@@ -4,6 +4,8 @@
 //
 // This file holds the C entries, the copies of operands that TMA cannot address
 // as they are, and the join of the vocabulary tiles.
+#include <atomic>
+
 #include "proj_common.cuh"
 #include "tc_ptx.cuh"
 
@@ -63,16 +65,16 @@ __global__ void __launch_bounds__(kJoinThreads) vocab_join_kernel(
 }
 
 int sm_count() {
-  static int count[64];
+  static std::atomic<int> count[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-  if (count[dev] == 0) {
-    int n = 0;
+  int n = count[dev].load();
+  if (n == 0) {
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0)
       n = 148;
-    count[dev] = n;
+    count[dev].store(n);
   }
-  return count[dev];
+  return n;
 }
 
 // ---- operands for TMA ----------------------------------------------------------

@@ -40,7 +40,10 @@ constexpr int kRawBytes = kTile * 128;       // one operand's slice as it arrive
 constexpr int kPartBytes = kTile * kSlice * 2;
 constexpr int kRawStages = 3, kPartStages = 2;
 constexpr int kRawStage = 2 * kRawBytes, kPartStage = 6 * kPartBytes;
-constexpr int kSplitSmem = kRawStages * kRawStage + kPartStages * kPartStage + 1024;
+// All of an SM's: this kernel takes all of TMEM, and its clusters must not meet
+// another kernel's on an SM where each would wait for what the other holds.
+constexpr int kSplitSmem = kSmemBudget;
+static_assert(kRawStages * kRawStage + kPartStages * kPartStage + 1024 <= kSplitSmem, "");
 constexpr int kSumSlices = 512 / kSlice;     // slices accumulated in TMEM at a time
 constexpr int kGatherWarps = 8, kGroupWarps = 4, kCopyWarp = 16, kIssueWarp = 17;
 // Registers per thread: at launch, and as the warpgroups share them out.
@@ -103,7 +106,9 @@ __device__ __forceinline__ float plain_dot(const Problem& p, const float* w, int
   const float* x = static_cast<const float*>(p.x) + row * p.x_rs;
   w += n * p.w_ns;
   float y = 0.f;
-  for (int k = 0; k < p.inner; ++k) y = fmaf(x[k], w[k * p.w_ks], y);
+  // a NaN stays one: a row of them ends at once
+  for (int k0 = 0; k0 < p.inner && y == y; k0 += 16)
+    for (int k = k0; k < min(k0 + 16, p.inner); ++k) y = fmaf(x[k], w[k * p.w_ks], y);
   return y;
 }
 

@@ -304,7 +304,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
     uint32_t n = 0;
     auto wait_acc = [&]() {
-      ok = __all_sync(kFullMask, tc::mbar_wait(&acc_full[n & 1], (n / 2) & 1, kWaitLimit));
+      ok = __all_sync(kFullMask,
+                      tc::mbar_wait(&acc_full[n & 1], (n / 2) & 1, whole_sum_limit(per_acc)));
       tc::tc_fence_after();
       return ok;
     };
@@ -422,6 +423,7 @@ struct StreamParams {
   int cols;    // activation rows rounded up to the instruction's 16
   int w_mn;
   int splits;  // CTAs per feature tile
+  int smem_bytes;
   int vec;     // four neighbouring outputs (biases, residuals) are 8 aligned bytes
 };
 
@@ -552,7 +554,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
   residual(row_first, r);
   float* sums = reinterpret_cast<float*>(smem);  // [op][row][feature], where the stages were
   if (warp < 4) {
-    ok = __all_sync(kFullMask, tc::mbar_wait(&acc_full, 0, kWaitLimit));
+    ok = __all_sync(kFullMask, tc::mbar_wait(&acc_full, 0, whole_sum_limit(kb1 - kb0)));
     tc::tc_fence_after();
     const uint32_t taddr = tmem + (static_cast<uint32_t>(warp) << 21);
     for (int c = 0; ok && c < p.rows; c += 16) {
@@ -706,7 +708,7 @@ int launch(const StreamParams& g, int tiles, cudaStream_t stream) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(tiles * g.splits));
   cfg.blockDim = dim3(kStreamThreads);
-  cfg.dynamicSmemBytes = g.stages * g.stage_bytes + 1024;
+  cfg.dynamicSmemBytes = g.smem_bytes;
   cfg.stream = stream;
   cudaLaunchAttribute attrs[2];
   cfg.attrs = attrs;
@@ -764,6 +766,12 @@ int run_stream(Kind kind, const Problem& p, int32_t dtype, int ctas, cudaStream_
   }
   const int per_cta = ceil_div(kblocks, g.splits);
   g.stages = budget / g.stage_bytes;
+  // The whole class even where less is used. CTAs of a cluster wait for one
+  // another, and TMEM is handed out as it comes: were more CTAs on an SM than its
+  // TMEM has room for, two clusters could each hold what the other waits for.
+  // With 110 KB two of these CTAs fit (256 of 512 columns), and none beside a
+  // cluster that takes all of TMEM, which asks for more than the other half.
+  g.smem_bytes = budget + 1024;
   if (g.stages > kStreamStages) g.stages = kStreamStages;
   if (g.stages > per_cta) g.stages = per_cta;
   const int sums = ops * g.cols * kStreamFeatures * 4;  // partial sums lie where the stages were

@@ -10,7 +10,8 @@ layer (:136-147), the recurrent core of all layers + final norm + exit gate
 captured core (vllm_rlt/worker/model_runner.py:386-431,
 vllm_rlt/worker/cuda_graph.py:43-122).
 
-GEMMs stay on cuBLAS (torch.matmul); the page write, the depth/page
+GEMMs run on cuBLAS (torch.matmul) or, with ``projections="kernels"``, on this
+package's projection kernels; the page write, the depth/page
 resolution, the decode attention and the LAST-EXITED exit copy run on the
 sm_100a kernels of this package. Weights are random (normal, std 0.02, as the
 reference's initialiser at models/ouro.py:183-191); no checkpoint is loaded.
@@ -32,6 +33,7 @@ import torch
 from .kernels import ouro_ops
 from .kernels.cache_ops import finalize, write_kv
 from .kernels.paged_attention import B200PagedAttention
+from .kernels.projections import gated_linear, greedy_tokens, linear
 from .kernels.routing import metadata
 
 
@@ -156,9 +158,18 @@ class OuroDecoder:
     """
 
     def __init__(self, shape: OuroShape, weights: OuroWeights, capacity, device, dtype,
-                 layout: str = "last_exited", page: int = 16, seed: int = 0, fused: bool = True):
+                 layout: str = "last_exited", page: int = 16, seed: int = 0, fused: bool = True,
+                 projections: str = "library"):
         self.shape, self.w = shape, weights
         self.fused = fused  # fused sm_100a glue kernels, or the plain torch expressions
+        # "library": torch.matmul and the steps after it, rounded one by one;
+        # "kernels": the projection kernels, which round once, and the sampled
+        # tokens' log-probabilities in ``logprobs``
+        if projections not in ("library", "kernels"):
+            raise ValueError('projections must be "library" or "kernels"')
+        if projections == "kernels" and not fused:
+            raise ValueError('projections="kernels" belongs to the fused layer')
+        self.projections = projections
         self.device, self.dtype, self.page = torch.device(device), dtype, page
         self.layout = layout
         self.planes = shape.loops if layout == "last_exited" else 1
@@ -189,6 +200,7 @@ class OuroDecoder:
         self.exit_mask = torch.zeros(n, device=self.device, dtype=torch.bool)
         self.start_mask = torch.zeros(n, device=self.device, dtype=torch.bool)
         self.tokens = torch.zeros(n, **i64)
+        self.logprobs = torch.zeros(n, device=self.device, dtype=torch.float32)
         self.hidden_state = torch.zeros((n, shape.hidden), device=self.device, dtype=dtype)
         # metadata produced on device by the routing kernel each step
         self.slot_ids = torch.zeros(n, **i64)
@@ -239,15 +251,20 @@ class OuroDecoder:
         this layer's normed input; returns (hidden, next_norm(hidden))."""
         s, w = self.shape, self.w
         norms = w.norms[index]
-        qkv = x @ w.wqkv[index].t()
+        own = self.projections == "kernels"
+        qkv = linear(x, w.wqkv[index]) if own else x @ w.wqkv[index].t()
         q = ouro_ops.rope_write_kv(qkv, self.positions, w.inv_freq, self.key_cache,
                                    self.value_cache, index, self.write_blocks,
                                    self.write_offsets, s.heads, s.kv_heads, s.head_dim)
         attn = self.attention(q, self.key_cache[:, index], self.value_cache[:, index],
                               self.row_tables, self.lengths)
-        out = attn.reshape(hidden.shape[0], -1) @ w.wo[index].t()
+        attn = attn.reshape(hidden.shape[0], -1)
+        out = linear(attn, w.wo[index]) if own else attn @ w.wo[index].t()
         hidden, x2 = ouro_ops.rms_norm(out, norms[1], s.eps, residual=hidden, weight2=norms[2])
-        mlp = ouro_ops.silu_mul(x2 @ w.wgu[index].t(), s.intermediate) @ w.wdown[index].t()
+        if own:
+            mlp = linear(gated_linear(x2, w.wgu[index]), w.wdown[index])
+        else:
+            mlp = ouro_ops.silu_mul(x2 @ w.wgu[index].t(), s.intermediate) @ w.wdown[index].t()
         return ouro_ops.rms_norm(mlp, norms[3], s.eps, residual=hidden, weight2=next_norm)
 
     def core(self, hidden):
@@ -265,8 +282,11 @@ class OuroDecoder:
             for index in range(layers):
                 hidden = self.layer(index, hidden, cos, sin)
             hidden = rms_norm(hidden, self.w.final_norm, self.shape.eps)
-        gate = torch.sigmoid(hidden @ self.w.gate_w.t() + self.w.gate_b).squeeze(-1)
-        return hidden, gate
+        if self.projections == "kernels":
+            gate = linear(hidden, self.w.gate_w, self.w.gate_b, activation="sigmoid")
+        else:
+            gate = torch.sigmoid(hidden @ self.w.gate_w.t() + self.w.gate_b)
+        return hidden, gate.squeeze(-1)
 
     # ------------------------------------------------------------- the step
 
@@ -281,8 +301,11 @@ class OuroDecoder:
         hidden, gate = self.core(hidden)
         if self.planes > 1:
             finalize(self.desc_exit, self.tables, self.key_cache, self.value_cache)
-        logits = hidden @ self.w.lm_head.t()
-        sampled = torch.argmax(logits, dim=-1)
+        if self.projections == "kernels":
+            sampled, logprobs = greedy_tokens(hidden, self.w.lm_head)
+            self.logprobs.copy_(torch.where(self.exit_mask, logprobs, self.logprobs))
+        else:
+            sampled = torch.argmax(hidden @ self.w.lm_head.t(), dim=-1)
         self.tokens.copy_(torch.where(self.exit_mask, sampled, self.tokens))
         self.hidden_state.copy_(hidden)
         self.gate = gate
@@ -292,7 +315,7 @@ class OuroDecoder:
         as vllm_rlt/worker/cuda_graph.py:95-112)."""
         # Warm-up passes rewrite the same KV slots the first real step writes,
         # but they also advance the sampled tokens and hidden states: restore.
-        saved = (self.tokens.clone(), self.hidden_state.clone())
+        saved = (self.tokens.clone(), self.hidden_state.clone(), self.logprobs.clone())
         stream = torch.cuda.Stream(self.device)
         stream.wait_stream(torch.cuda.current_stream(self.device))
         with torch.cuda.stream(stream):
@@ -302,6 +325,7 @@ class OuroDecoder:
         torch.cuda.synchronize(self.device)
         self.tokens.copy_(saved[0])
         self.hidden_state.copy_(saved[1])
+        self.logprobs.copy_(saved[2])
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):
             self.step_body()
