@@ -146,6 +146,42 @@ __device__ __forceinline__ VocabPart vocab_part(const Problem& p, const float (&
   return part;
 }
 
+// The record of a row's 128 logits in one vocabulary tile, four to a lane from
+// entry n on, written as the row's record `tile`. For a whole warp.
+__device__ __forceinline__ void vocab_row(const Problem& p, const float (&l)[4], int row, int n,
+                                          int tile) {
+  VocabPart part{-INFINITY, 0.f, INT32_MAX, 0.f};
+  const int64_t want = p.tokens != nullptr ? p.tokens[row] : -1;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (n + e >= p.outer) continue;
+    if (beats(l[e], n + e, part.most, part.at)) {
+      part.most = l[e];
+      part.at = n + e;
+    }
+    if (n + e == want) part.chosen = l[e];
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float m = __shfl_xor_sync(kFullMask, part.most, o);
+    const int at = __shfl_xor_sync(kFullMask, part.at, o);
+    if (beats(m, at, part.most, part.at)) {
+      part.most = m;
+      part.at = at;
+    }
+    part.chosen += __shfl_xor_sync(kFullMask, part.chosen, o);
+  }
+  const float base = part.most == -INFINITY ? 0.f : part.most;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (n + e < p.outer) part.sum += ex2((l[e] - base) * kLog2e);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) part.sum += __shfl_xor_sync(kFullMask, part.sum, o);
+  if ((threadIdx.x & 31) == 0)
+    *reinterpret_cast<float4*>(&p.parts[static_cast<int64_t>(row) * p.tiles + tile]) =
+        make_float4(part.most, part.sum, __int_as_float(part.at), part.chosen);
+}
+
 // ---- host side ----
 
 inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {

@@ -623,11 +623,15 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
       tc::cluster_arrive(all);
       arrived = true;
     }
-    float next[4];
-    residual(row + row_step, next);
-    if (n < p.outer) finish4<T, kKind, kAct>(p, g.vec, row, n, y[0], y[kOps - 1], b, r);
+    if constexpr (kKind == kVocab) {
+      vocab_row(p, y[0], row, n, n0 / kStreamFeatures);
+    } else {
+      float next[4];
+      residual(row + row_step, next);
+      if (n < p.outer) finish4<T, kKind, kAct>(p, g.vec, row, n, y[0], y[kOps - 1], b, r);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) r[e] = next[e];
+      for (int e = 0; e < 4; ++e) r[e] = next[e];
+    }
   }
   __syncwarp();
   if (g.splits > 1) {
@@ -722,17 +726,15 @@ int by_type(const Params& g, int32_t dtype, int ctas, cudaStream_t stream) {
                            : by_activation<kKind, __half>(g, ctas, stream);
 }
 
-int run_stream(Kind kind, const Problem& p, int32_t dtype, int ctas, cudaStream_t stream) {
-  StreamParams g{};
-  const int ops = kind == kGated ? 2 : 1;
-  g.p = p;
-  g.w_mn = p.w_ks != 1;
-  g.cols = ceil_div(p.rows, 16) * 16;
-  g.vec = p.outer % 4 == 0 && p.o_rs % 4 == 0 && p.r_rs % 4 == 0 && aligned_to(p.out, 8) &&
-          aligned_to(p.bias, 8) && aligned_to(p.residual, 8);
-  g.stage_bytes = ops * kStreamFeatures * kBlockK * 2 + g.cols * 128;
+struct StreamPlan {
+  int splits;  // CTAs per tile
+  int budget;  // shared memory of a CTA's stages
+};
+
+StreamPlan stream_plan(const Problem& p, int ctas) {
   const int tiles = ceil_div(p.outer, kStreamFeatures);
   const int kblocks = ceil_div(p.inner, kBlockK);
+  StreamPlan plan{1, 110 * 1024};
   // CTAs per tile and shared memory per CTA: the least weights per SM, where
   // either one CTA of 200 KB runs on an SM (its clusters then have to fit the
   // die's parts) or two of 110 KB. The partial sums of many rows cost more to
@@ -742,7 +744,6 @@ int run_stream(Kind kind, const Problem& p, int32_t dtype, int ctas, cudaStream_
   const bool many = p.rows > 16;
   constexpr int kBig = 200 * 1024, kSmall = 110 * 1024;
   double least = 1e300;
-  int budget = kSmall;
   for (int s = 1; s <= kMaxSplits && s <= kblocks; ++s) {
     for (int big = 0; big < 2; ++big) {
       constexpr auto kernel = stream_kernel<__half, kLinear, RLT_ACT_NONE>;
@@ -759,19 +760,44 @@ int run_stream(Kind kind, const Problem& p, int32_t dtype, int ctas, cudaStream_
       const double cost = static_cast<double>(waves) / s * (big == many ? 1.0 : 1.5);
       if (cost < least * (many ? 0.999 : 1.001)) {
         least = cost;
-        g.splits = s;
-        budget = big ? kBig : kSmall;
+        plan.splits = s;
+        plan.budget = big ? kBig : kSmall;
       }
     }
   }
+  return plan;
+}
+
+// Whether the vocabulary head streams too: few rows, and so few tiles that a
+// cluster shares each. A CTA's sums then cover at most kVocabBlocks blocks of
+// input features (half as many again where that is the last split), as they do
+// in gemm_kernel.
+bool head_streams(const Problem& p, int ctas) {
+  return p.rows <= kStreamRows && ceil_div(ceil_div(p.inner, kBlockK), stream_plan(p, ctas).splits) <=
+                                      kVocabBlocks + kVocabBlocks / 2;
+}
+
+int run_stream(Kind kind, const Problem& p, int32_t dtype, int ctas, cudaStream_t stream) {
+  StreamParams g{};
+  const int ops = kind == kGated ? 2 : 1;
+  g.p = p;
+  g.w_mn = p.w_ks != 1;
+  g.cols = ceil_div(p.rows, 16) * 16;
+  g.vec = p.outer % 4 == 0 && p.o_rs % 4 == 0 && p.r_rs % 4 == 0 && aligned_to(p.out, 8) &&
+          aligned_to(p.bias, 8) && aligned_to(p.residual, 8);
+  g.stage_bytes = ops * kStreamFeatures * kBlockK * 2 + g.cols * 128;
+  const int tiles = ceil_div(p.outer, kStreamFeatures);
+  const StreamPlan plan = stream_plan(p, ctas);
+  g.splits = plan.splits;
+  const int kblocks = ceil_div(p.inner, kBlockK);
   const int per_cta = ceil_div(kblocks, g.splits);
-  g.stages = budget / g.stage_bytes;
+  g.stages = plan.budget / g.stage_bytes;
   // The whole class even where less is used. CTAs of a cluster wait for one
   // another, and TMEM is handed out as it comes: were more CTAs on an SM than its
   // TMEM has room for, two clusters could each hold what the other waits for.
   // With 110 KB two of these CTAs fit (256 of 512 columns), and none beside a
   // cluster that takes all of TMEM, which asks for more than the other half.
-  g.smem_bytes = budget + 1024;
+  g.smem_bytes = plan.budget + 1024;
   if (g.stages > kStreamStages) g.stages = kStreamStages;
   if (g.stages > per_cta) g.stages = per_cta;
   const int sums = ops * g.cols * kStreamFeatures * 4;  // partial sums lie where the stages were
@@ -784,18 +810,23 @@ int run_stream(Kind kind, const Problem& p, int32_t dtype, int ctas, cudaStream_
                        : encode2d(map, dtype, base, p.inner, p.outer, p.w_ns, kStreamFeatures));
   }
   if (!ok) return RLT_E_DEVICE;
-  return kind == kGated ? by_type<kGated>(g, dtype, tiles, stream)
-                        : by_type<kLinear>(g, dtype, tiles, stream);
+  switch (kind) {
+    case kLinear: return by_type<kLinear>(g, dtype, tiles, stream);
+    case kGated: return by_type<kGated>(g, dtype, tiles, stream);
+    default: return by_type<kVocab>(g, dtype, tiles, stream);
+  }
 }
 
 }  // namespace
 
 int tc_vocab_parts(const Problem& p, int ctas) {
+  if (head_streams(p, ctas)) return ceil_div(p.outer, kStreamFeatures);
   return 2 * ceil_div(p.outer, choose_tiling(kVocab, p, ctas).set_n);
 }
 
 int run_tc(Kind kind, const Problem& p, int32_t dtype, int ctas, cudaStream_t stream) {
-  if (kind != kVocab && p.rows <= kStreamRows) return run_stream(kind, p, dtype, ctas, stream);
+  if (kind == kVocab ? head_streams(p, ctas) : p.rows <= kStreamRows)
+    return run_stream(kind, p, dtype, ctas, stream);
   GemmParams g{};
   g.p = p;
   const Tiling tiling = choose_tiling(kind, p, ctas);
