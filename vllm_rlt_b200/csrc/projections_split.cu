@@ -482,13 +482,16 @@ int run_split(Kind kind, const Problem& p, int ctas, cudaStream_t stream) {
   const int64_t tiles = static_cast<int64_t>(g.row_tiles) * ceil_div(p.outer, set);
   const int slices = ceil_div(p.inner, kSlice);
   // CTAs per tile: one CTA fits an SM, so what counts is how many clusters run
-  // at once. In slices' times; a CTA pays about eight for its start and end.
+  // at once. In slices' times; a CTA pays about eight for its start and end. The
+  // head, whose rows need no exchange in one CTA, has to gain half as much again
+  // (600 rows of 2112 against 16496 entries: 269 us, in pairs 366).
   g.splits = 1;
-  int64_t least = INT64_MAX;
+  double least = 1e300;
   for (int s = 1; s <= kMaxSplits && slices >= 4 * s; ++s) {
     constexpr auto kernel = split_kernel<float, kLinear, RLT_ACT_NONE>;
     const int64_t at_once = s == 1 ? ctas : resident_clusters<kernel>(s, kSplitThreads, kSplitSmem);
-    const int64_t cost = (tiles + at_once - 1) / at_once * (ceil_div(slices, s) + 8);
+    const double cost = static_cast<double>((tiles + at_once - 1) / at_once) *
+                        (ceil_div(slices, s) + 8) * (kind == kVocab && s > 1 ? 1.5 : 1.0);
     if (cost < least) {
       least = cost;
       g.splits = s;
