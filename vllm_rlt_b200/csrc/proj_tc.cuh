@@ -106,22 +106,40 @@ __device__ __forceinline__ VocabPart vocab_part(const Problem& p, const float (&
                                                 int cols, int64_t want) {
   VocabPart part{-INFINITY, 0.f, INT32_MAX, 0.f};
   if (cols <= 0) return part;
+  // Sum of 2^(l log2e - b) with b = most * log2e rounded: one multiply-add and
+  // one exponential per logit. b's rounding is the same in every term, and taken
+  // back as a factor at the end.
+  if (cols == kN) {  // the whole of a full tile: no test per column
 #pragma unroll
-  for (int c = 0; c < kN; c += 16)
-    if (c < cols)
+    for (int j = 0; j < kN; ++j) part.most = fmaxf(part.most, v[j]);
+  } else {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) part.most = fmaxf(part.most, c + j < cols ? v[c + j] : -INFINITY);
+    for (int c = 0; c < kN; c += 16)
+      if (c < cols)
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          part.most = fmaxf(part.most, c + j < cols ? v[c + j] : -INFINITY);
+  }
   const float base = part.most == -INFINITY ? 0.f : part.most;
+  const float b = base * kLog2e;
   float s0 = 0.f, s1 = 0.f;
+  if (cols == kN) {
 #pragma unroll
-  for (int c = 0; c < kN; c += 16)
-    if (c < cols)
+    for (int j = 0; j < kN; j += 2) {
+      s0 += ex2(fmaf(v[j], kLog2e, -b));
+      s1 += ex2(fmaf(v[j + 1], kLog2e, -b));
+    }
+  } else {
 #pragma unroll
-      for (int j = 0; j < 16; j += 2) {
-        s0 += c + j < cols ? ex2((v[c + j] - base) * kLog2e) : 0.f;
-        s1 += c + j + 1 < cols ? ex2((v[c + j + 1] - base) * kLog2e) : 0.f;
-      }
-  part.sum = s0 + s1;
+    for (int c = 0; c < kN; c += 16)
+      if (c < cols)
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) {
+          s0 += c + j < cols ? ex2(fmaf(v[c + j], kLog2e, -b)) : 0.f;
+          s1 += c + j + 1 < cols ? ex2(fmaf(v[c + j + 1], kLog2e, -b)) : 0.f;
+        }
+  }
+  part.sum = (s0 + s1) * ex2(-fmaf(base, kLog2e, -b));
   if (p.tokens != nullptr) {
     const bool here = want >= n0 && want < n0 + cols;
     if (__any_sync(kFullMask, here)) {
