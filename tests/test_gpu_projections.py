@@ -479,7 +479,7 @@ def test_offsets_beyond_32_bits(dtype):
     w = normal(g, 64, 128, std=0.05, dtype=dtype)
     rb.linear(x, w, residual=residual, out=out)
     assert_within(out, *po.linear(x, w, residual=residual))
-    head = room.as_strided((4, 128), (gap, 1), 3072)  # weights far apart as well
+    head = room.as_strided((4, 128), (gap, 1), 3200)  # weights far apart as well
     head.copy_(normal(g, 4, 128))
     assert_within(rb.linear(x, head), *po.linear(x, head))
 

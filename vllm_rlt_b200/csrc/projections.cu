@@ -130,18 +130,26 @@ __global__ void __launch_bounds__(256) align_kernel(const U* __restrict__ src,
                                                     int64_t stride, int pitch) {
   constexpr int kUnit = 16 / sizeof(U);
   const int units = pitch / kUnit;
-  const int64_t total = static_cast<int64_t>(units) * lines;
-  for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
-    const int64_t line = i / units;
-    const int c = static_cast<int>(i - line * units) * kUnit;
-    const U* s = src + line * stride + c;
-    union {
-      U v[kUnit];
-      uint4 all;
-    } t;
+  // a warp takes 128 units of a line at a time
+  const uint32_t chunks = (units + 127) / 128, lane = threadIdx.x & 31;
+  const int64_t items = static_cast<int64_t>(chunks) * lines;
+  for (int64_t item = blockIdx.x * 8LL + (threadIdx.x >> 5); item < items; item += gridDim.x * 8LL) {
+    const int64_t line = items <= UINT32_MAX ? static_cast<uint32_t>(item) / chunks : item / chunks;
+    const int first = static_cast<int>(item - line * chunks) * 128 + lane;
+    const U* s = src + line * stride;
+    U* d = dst + line * pitch;
 #pragma unroll
-    for (int e = 0; e < kUnit; ++e) t.v[e] = c + e < length ? s[e] : static_cast<U>(0);
-    st_vec(dst + line * pitch + c, t.all);
+    for (int q = 0; q < 4; ++q) {
+      const int c = (first + q * 32) * kUnit;
+      if (c >= pitch) continue;
+      union {
+        U v[kUnit];
+        uint4 all;
+      } t;
+#pragma unroll
+      for (int e = 0; e < kUnit; ++e) t.v[e] = c + e < length ? s[c + e] : static_cast<U>(0);
+      st_vec(d + c, t.all);
+    }
   }
 }
 
@@ -149,7 +157,7 @@ int align_copy(const void*& base, int64_t& stride, int length, int lines, int32_
                cudaStream_t stream) {
   const int64_t pitch = padded(length, dtype);
   if (pitch > INT32_MAX) return RLT_E_SHAPE;
-  const int64_t blocks = (pitch * elem_bytes(dtype) / 16 * lines + 255) / 256;
+  const int64_t blocks = ((pitch * elem_bytes(dtype) / 16 + 127) / 128 * lines + 7) / 8;
   const unsigned grid =
       static_cast<unsigned>(blocks < 16 * sm_count() ? blocks : 16 * sm_count());
   if (dtype == RLT_F32)
