@@ -72,18 +72,6 @@ __device__ __forceinline__ float activate(float x) {
   return x;
 }
 
-template <bool kPrecise>
-__device__ __forceinline__ float activate(int act, float x) {
-  switch (act) {
-    case RLT_ACT_SILU: return activate<kPrecise, RLT_ACT_SILU>(x);
-    case RLT_ACT_GELU: return activate<kPrecise, RLT_ACT_GELU>(x);
-    case RLT_ACT_GELU_TANH: return activate<kPrecise, RLT_ACT_GELU_TANH>(x);
-    case RLT_ACT_RELU: return activate<kPrecise, RLT_ACT_RELU>(x);
-    case RLT_ACT_SIGMOID: return activate<kPrecise, RLT_ACT_SIGMOID>(x);
-    default: return x;
-  }
-}
-
 // Whether logit b at vocabulary entry j beats a at i: larger, or NaN as torch's
 // argmax orders it (above every number), the lower entry on a tie.
 __device__ __forceinline__ bool beats(float b, int j, float a, int i) {
