@@ -502,3 +502,44 @@ def test_a_row_of_infinities_and_not_numbers_in_single_precision():
         close = po.linear(torch.nan_to_num(x, 0, 0, 0), torch.nan_to_num(w, 0, 0, 0))
         off = (got.double() - close[0]).abs() - close[1]
         assert bool((off[fine] <= 0).all())
+
+
+@pytest.mark.parametrize("rows", [4, 200])
+def test_captured_behind_copies_and_other_streams(rows):
+    """In a captured graph the kernels follow memory copies, memsets, kernels of
+    other libraries and a joined side stream, and read what those wrote."""
+    g = generator(71)
+    source = normal(g, rows, 256, dtype=torch.bfloat16)
+    x, y = torch.zeros_like(source), torch.zeros_like(source)
+    w = normal(g, 256, 256, std=0.05, dtype=torch.bfloat16)
+    v = torch.empty_like(w)
+    side = torch.cuda.Stream()
+
+    def work():
+        x.copy_(source)  # a copy of device memory
+        a = rb.linear(x, w)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            y.copy_(source)
+            b = rb.gated_linear(y, w)
+        v.zero_()
+        v.add_(w)  # weights written by the kernel just before
+        c = rb.linear(x, v, residual=a)
+        torch.cuda.current_stream().wait_stream(side)
+        d = rb.linear(b, v[:, :128].contiguous())
+        x.zero_()  # after their last reader
+        y.zero_()
+        return a, b, c, d, *rb.greedy_tokens(a, v)
+
+    want = [t.clone() for t in work()]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = work()
+    for _ in range(20):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    for _ in range(20):  # and eagerly, without a wait in between
+        got = work()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
