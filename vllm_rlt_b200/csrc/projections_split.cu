@@ -155,6 +155,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     aborted = 0;
     tc::fence_mbar_init();
   }
+  __syncwarp();
   if (warp == kIssueWarp) tc::tmem_alloc(&tmem_slot, 512);
   tc::tc_fence_before();
   __syncthreads();
@@ -384,6 +385,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
       read4<float>(bias_at != nullptr && n < p.outer ? bias_at + n : nullptr, g.vec, p.outer - n,
                    bias);
       residual(row_first, add);
+      __syncwarp();  // its reads differ by lane; the barrier wants whole warps
       if (g.splits > 1)
         tc::cluster_sync();
       else

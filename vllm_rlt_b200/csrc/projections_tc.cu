@@ -177,6 +177,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     aborted = 0;
     tc::fence_mbar_init();
   }
+  __syncwarp();  // the cluster's barrier wants whole warps
   if (warp == kEpilogueWarps + 1) {
     if (kPair)
       tc::tmem_alloc_pair(&tmem_slot, 512);
@@ -458,6 +459,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
     aborted = 0;
     tc::fence_mbar_init();
   }
+  __syncwarp();
   if (warp == 5) tc::tmem_alloc(&tmem_slot, kTmemCols);
   if (warp == 4 && tc::elect_one()) {
     for (int kb = kb0; kb < min(kb1, kb0 + kStreamAhead); ++kb)
