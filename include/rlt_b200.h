@@ -415,7 +415,8 @@ size_t rlt_linear_workspace_bytes(const void* x, const void* weight, int32_t dty
 
 /* Matrix product with its epilogue, in one launch:
  *   out[r, n] = act(sum_k x[r, k] weight[n, k] + bias[n]) + residual[r, n]
- * accumulated in fp32 and rounded once to the dtype. weight is [out, in] with
+ * accumulated in fp32 (on the tensor cores, which truncate, at most 768 input
+ * features at a time) and rounded once to the dtype. weight is [out, in] with
  * either dimension contiguous (weight_in_stride 1, or weight_out_stride 1: the
  * transposed view of an [in, out] tensor); the last dimension of x, residual
  * and out is contiguous. bias and residual may be NULL; out may be the same

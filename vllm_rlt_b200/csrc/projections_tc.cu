@@ -12,14 +12,18 @@
 // by itself, (128 + N / 2) x 128 for one of a pair (each holds half of the
 // weights' slice). At N = 256 that is 819 and 546 cycles against 512, so wide
 // tiles on pairs are the ones near the tensor cores' rate: 4096 x 2048 -> 2 x 5632
-// takes 122 us, 1,550 TFLOP/s with the tensor pipe 90 % active.
+// takes 127 us, 1,490 TFLOP/s.
 //
 // A thread of warps 0-7 holds one activation row of the tile (its TMEM lane)
 // and half of its columns, so the vocabulary head's maximum and sum need no
-// exchange between threads. The tensor core truncates as it accumulates (an
-// error of one sign that grows with the number of k-steps), so the head, whose
-// outputs are fp32, accumulates at most 512 input features in TMEM and adds
-// those sums in registers, rounded to nearest.
+// exchange between threads. The tensor core truncates as it accumulates, an
+// error of one sign that grows with the number of steps: over 16384 features of
+// one sign a sum in TMEM came out 1.07e-4 too small (fp16; bf16 8.2e-5). So at
+// most 768 input features are accumulated there (512 for the head, whose outputs
+// are fp32), and those sums are added in registers, rounded to nearest: 4e-6 at
+// any length. Of 4096 x 5632 -> 2048 in bf16, 5.0e-4 of the outputs then differ
+// from the rounded exact ones, as with fp32 products rounded to nearest (4.5e-4),
+// and 3.2e-3 did before.
 //
 // Weights may have either dimension contiguous: with the input features
 // contiguous a stage holds them K-major (128-byte rows of 64 input features),
@@ -29,11 +33,11 @@
 // stream_kernel: few activation rows. The weights are what has to be read, so
 // here they are the 128-row operand and the activations the narrow one (16 to
 // 64 columns): a CTA streams 128 output features over its share of the input
-// features, a cluster of up to 8 CTAs shares a feature tile, and their partial
-// sums meet in distributed shared memory: each CTA reads the others' for the
-// rows that it finishes (stored there by the others with st.async instead, 64
-// rows took 9.4 us where reading takes 7.9). While the stream's previous kernel
-// still runs, the first weights are brought into L2.
+// features in TMEM accumulators of at most 512 of them, a cluster of up to 8 CTAs
+// shares a feature tile, and their partial sums meet in distributed shared memory:
+// each CTA reads the others' for the rows that it finishes (stored there by the
+// others with st.async instead, 64 rows took 9.4 us where reading takes 7.9). While
+// the stream's previous kernel still runs, the first weights are brought into L2.
 #include "proj_tc.cuh"
 
 namespace rlt {
@@ -45,13 +49,17 @@ constexpr int kTileM = 128;                    // activation rows per CTA
 constexpr int kMaxStages = 10;
 constexpr int kEpilogueWarps = 8;
 // Warps 8 and 9 copy and multiply; 10 and 11 complete their warpgroup. The
-// head's epilogue threads hold 128 sums each and take registers from it.
+// epilogue threads hold 128 sums each and take registers from it.
 constexpr int kThreads = (kEpilogueWarps + 4) * 32;
-constexpr int kLaunchRegs = 168, kSumRegs = 232, kOtherRegs = 40;  // per thread, the head's kernel
+constexpr int kLaunchRegs = 168, kSumRegs = 232, kOtherRegs = 40;  // per thread
 static_assert(256 * kSumRegs + 128 * kOtherRegs <= kThreads * kLaunchRegs,
               "the increase draws on what the launch allocated");
 constexpr int kStagingBytes = kEpilogueWarps * 4096;  // 32 rows x 32 fp32 columns per warp
-constexpr int kVocabBlocks = 8;  // 64-feature blocks accumulated in TMEM at a time by the head
+// 64-feature blocks accumulated in TMEM at a time: by the head and few rows, and
+// by the other tiles. With 8 the latter's next tile waits for the two accumulators
+// while outputs are stored: 4096 x 5632 -> 2048 takes 78.9 us, the gated product
+// 4096 x 2048 -> 2 x 5632 136; with 12, 75.8 and 127; with 16, 73.9 and 124.
+constexpr int kSumBlocks = 8, kTileSumBlocks = 12;
 
 struct GemmParams {
   CUtensorMap map_x, map_w, map_up;
@@ -103,25 +111,33 @@ __device__ __forceinline__ void finish32(const Problem& p, int vec, uint8_t* sta
     float b[4] = {0.f, 0.f, 0.f, 0.f};
     uint2 r[8];  // the residuals, on their way together
     if (bias != nullptr) load4<T>(bias + at, b);
-    if (res != nullptr)
+    if (res != nullptr)  // past the last row, that one's again: a test per load would part them
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (i * 4 + (lane >> 3) < rows)
-          r[i] = *reinterpret_cast<const uint2*>(res + (row0 + i * 4 + (lane >> 3)) * p.r_rs + at);
+        r[i] = *reinterpret_cast<const uint2*>(
+            res + (row0 + min(i * 4 + (lane >> 3), rows - 1)) * p.r_rs + at);
     __syncwarp();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int row = i * 4 + (lane >> 3);
-      if (row >= rows) continue;
-      const float4 f =
-          *reinterpret_cast<const float4*>(staging + row * 128 + ((c ^ (row & 7)) << 4));
-      float y[4] = {f.x, f.y, f.z, f.w};
-      float add[4] = {0.f, 0.f, 0.f, 0.f};
-      if (res != nullptr) widen4<T>(r[i], add);
-      T o[4];
+    for (int i0 = 0; i0 < 8; i0 += 4) {
+      float4 f[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = from_f32<T>(activate<false, kAct>(y[e] + b[e]) + add[e]);
-      *reinterpret_cast<uint2*>(out + (row0 + row) * p.o_rs + at) = *reinterpret_cast<uint2*>(o);
+      for (int i = 0; i < 4; ++i) {
+        const int row = (i0 + i) * 4 + (lane >> 3);
+        f[i] = *reinterpret_cast<const float4*>(staging + row * 128 + ((c ^ (row & 7)) << 4));
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = (i0 + i) * 4 + (lane >> 3);
+        float y[4] = {f[i].x, f[i].y, f[i].z, f[i].w};
+        float add[4] = {0.f, 0.f, 0.f, 0.f};
+        if (res != nullptr) widen4<T>(r[i0 + i], add);
+        T o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          o[e] = from_f32<T>(activate<false, kAct>(y[e] + b[e]) + add[e]);
+        if (row < rows)
+          *reinterpret_cast<uint2*>(out + (row0 + row) * p.o_rs + at) = *reinterpret_cast<uint2*>(o);
+      }
     }
   } else {  // one column per lane
     __syncwarp();
@@ -196,12 +212,12 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
 
   const int kblocks = (p.inner + kBlockK - 1) / kBlockK;
   const int tiles = g.row_tiles * g.col_tiles;
+  constexpr int kPerAcc = kKind == kVocab ? kSumBlocks : kTileSumBlocks;
   const int first = blockIdx.x / kCtas, step = gridDim.x / kCtas;
-  const int per_acc = kKind == kVocab ? kVocabBlocks : kblocks;  // blocks per accumulator
   bool ok = true;
 
   if (warp >= kEpilogueWarps) {
-    if constexpr (kKind == kVocab) tc::setmaxnreg_dec<kOtherRegs>();
+    tc::setmaxnreg_dec<kOtherRegs>();
     if (warp == kEpilogueWarps) {
       const bool both = kKind == kGated && !kPair;  // this CTA copies gate and up rows
       const uint32_t bytes = (g.box_m + g.load_n * (both ? 2 : 1)) * 128 * kCtas;
@@ -263,7 +279,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
           }
           tc::tc_fence_after();
           const uint32_t d = tmem + acc.slot * 256;
-          const int kb_end = min(kb + per_acc, kblocks);
+          const int kb_end = min(kb + kPerAcc, kblocks);
           for (uint32_t more = 0; kb < kb_end; ++kb, at.next(g.stages)) {
             if (!__all_sync(kFullMask, tc::mbar_poll(&full[at.slot], at.parity, kWaitLimit))) {
               ok = false;
@@ -300,14 +316,14 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
       }
     }
   } else {
-    if constexpr (kKind == kVocab) tc::setmaxnreg_inc<kSumRegs>();
+    tc::setmaxnreg_inc<kSumRegs>();
     uint8_t* staging = smem + warp * 4096;
     const int half = warp >> 2;  // this thread's columns
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
     uint32_t n = 0;
     auto wait_acc = [&]() {
       ok = __all_sync(kFullMask,
-                      tc::mbar_wait(&acc_full[n & 1], (n / 2) & 1, whole_sum_limit(per_acc)));
+                      tc::mbar_wait(&acc_full[n & 1], (n / 2) & 1, whole_sum_limit(kPerAcc)));
       tc::tc_fence_after();
       return ok;
     };
@@ -329,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
       if constexpr (kKind == kVocab) {
         const int mine = g.tile_n / 2;  // a multiple of 16, at most 128
         float v[128];
-        for (int kb = 0; kb < kblocks; kb += kVocabBlocks) {
+        for (int kb = 0; kb < kblocks; kb += kSumBlocks) {
           if (!wait_acc()) break;
           const uint32_t taddr = tmem + (n & 1) * 256 + lanes + half * mine;
 #pragma unroll
@@ -354,33 +370,51 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
               &p.parts[static_cast<int64_t>(row) * p.tiles + col_tile * 2 + half]) =
               make_float4(part.most, part.sum, __int_as_float(part.at), part.chosen);
       } else {
-        if (!wait_acc()) break;
-        const uint32_t taddr = tmem + (n & 1) * 256 + lanes;
+        // chunks of 32 features 64 apart: four of them, or two of gate and two of up
+        constexpr int kChunks = kKind == kGated ? 2 : 4;
         const int end = min(p.outer, n0 + g.set_n);
-        if (row0 < p.rows) {
-          for (int c = half * 32; c < end - n0; c += 64) {
-            uint32_t t[32];
-            float v[32];
-            __syncwarp();
-            tc::tmem_ld32(taddr + c, t);
-            if constexpr (kKind == kGated) {
-              uint32_t up[32];
-              tc::tmem_ld32(taddr + g.set_n + c, up);
-              tc::tmem_ld_wait(t);
-              tc::tmem_ld_wait(up);
+        const int cols = row0 < p.rows ? end - n0 : 0;
+        float v[4][32];
+        for (int kb = 0; kb < kblocks; kb += kPerAcc) {
+          if (!wait_acc()) break;
+          const uint32_t taddr = tmem + (n & 1) * 256 + lanes;
 #pragma unroll
-              for (int j = 0; j < 32; ++j)
-                v[j] = activate<false, kAct>(__uint_as_float(t[j])) * __uint_as_float(up[j]);
-              finish32<T, RLT_ACT_NONE>(p, g.vec, staging, row0, n0 + c, end, v);
-            } else {
-              tc::tmem_ld_wait(t);
+          for (int j = 0; j < 4; ++j) {
+            const int c = half * 32 + j % kChunks * 64;
+            if (c < cols) {
+              __syncwarp();
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(t[j]);
-              finish32<T, kAct>(p, g.vec, staging, row0, n0 + c, end, v);
+              for (int i0 = 0; i0 < 32; i0 += 16) {
+                uint32_t t[16];
+                tc::tmem_ld16(taddr + j / kChunks * g.set_n + c + i0, t);
+                tc::tmem_ld_wait(t);
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                  v[j][i0 + i] =
+                      kb == 0 ? __uint_as_float(t[i]) : v[j][i0 + i] + __uint_as_float(t[i]);
+              }
             }
           }
+          release_acc();
         }
-        release_acc();
+        if (!ok) break;
+        // one copy of the code that finishes a chunk (unrolled, its instructions
+        // take longer to arrive than to run): the sums move up instead
+#pragma unroll 1
+        for (int c = half * 32; c < cols; c += 64) {
+          if constexpr (kKind == kGated) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              v[0][i] = activate<false, kAct>(v[0][i]) * v[kChunks][i];
+            finish32<T, RLT_ACT_NONE>(p, g.vec, staging, row0, n0 + c, end, v[0]);
+          } else {
+            finish32<T, kAct>(p, g.vec, staging, row0, n0 + c, end, v[0]);
+          }
+#pragma unroll
+          for (int j = 0; j < 3; ++j)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[j][i] = v[j + 1][i];
+        }
       }
     }
   }
@@ -414,6 +448,7 @@ constexpr int kStreamThreads = 384;
 constexpr int kStreamRows = 64;     // activation rows that stream_kernel takes
 constexpr int kStreamStages = 12;
 constexpr int kStreamFeatures = 128;
+constexpr int kStreamTmem = 256;    // columns of a CTA: its accumulators
 
 constexpr int kStreamAhead = 16;  // blocks of weights brought into L2 ahead of time
 
@@ -427,6 +462,8 @@ struct StreamParams {
   int splits;  // CTAs per feature tile
   int smem_bytes;
   int vec;     // four neighbouring outputs (biases, residuals) are 8 aligned bytes
+  int acc_blocks;  // blocks per accumulator
+  int acc_cols;    // TMEM columns between accumulators
 };
 
 template <typename T, Kind kKind, int kAct>
@@ -445,7 +482,6 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
   const int kblocks = (p.inner + kBlockK - 1) / kBlockK;
   const int kb0 = static_cast<int>(static_cast<int64_t>(kblocks) * rank / g.splits);
   const int kb1 = static_cast<int>(static_cast<int64_t>(kblocks) * (rank + 1) / g.splits);
-  constexpr uint32_t kTmemCols = kOps * kStreamRows;  // 64 or 128, powers of two
 
   if (threadIdx.x == 128) {
     tc::prefetch_tensormap(&g.map_w);
@@ -460,7 +496,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
     tc::fence_mbar_init();
   }
   __syncwarp();
-  if (warp == 5) tc::tmem_alloc(&tmem_slot, kTmemCols);
+  if (warp == 5) tc::tmem_alloc(&tmem_slot, kStreamTmem);
   if (warp == 4 && tc::elect_one()) {
     for (int kb = kb0; kb < min(kb1, kb0 + kStreamAhead); ++kb)
 #pragma unroll
@@ -518,8 +554,14 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
     const uint32_t w_hi = static_cast<uint32_t>(w_desc >> 32);
     const uint32_t x_hi = static_cast<uint32_t>(x_desc >> 32);
     Ring at;
-    uint32_t more = 0;
+    uint32_t d = tmem, more = 0;
+    int left = g.acc_blocks;  // of the present accumulator
     for (int kb = kb0; kb < kb1; ++kb, at.next(g.stages)) {
+      if (left-- == 0) {
+        left = g.acc_blocks - 1;
+        d += kOps * g.acc_cols;
+        more = 0;
+      }
       if (!__all_sync(kFullMask, tc::mbar_poll(&full[at.slot], at.parity, kWaitLimit))) {
         ok = false;
         break;
@@ -532,7 +574,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
         for (int ks = 0; ks < kBlockK / 16; ++ks)
 #pragma unroll
           for (int op = 0; op < kOps; ++op)
-            tc::mma_f16_ss(tmem + op * kStreamRows,
+            tc::mma_f16_ss(d + op * g.acc_cols,
                            tc::desc64(w_lo + op * (kBytesW >> 4) + ks * kstep_w, w_hi),
                            tc::desc64(x_lo + ks * 2, x_hi), idesc, ks > 0 ? 1 : more);
         tc::mma_commit(&empty[at.slot]);
@@ -565,12 +607,20 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
 #pragma unroll
       for (int op = 0; op < kOps; ++op) {
         uint32_t v[16];
+        float y[16];
         __syncwarp();
-        tc::tmem_ld16(taddr + op * kStreamRows + c, v);
+        tc::tmem_ld16(taddr + op * g.acc_cols + c, v);
         tc::tmem_ld_wait(v);
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-          at[(op * g.cols + j) * kStreamFeatures] = __uint_as_float(v[j]);
+        for (int j = 0; j < 16; ++j) y[j] = __uint_as_float(v[j]);
+        for (int a = 1; a * g.acc_blocks < kb1 - kb0; ++a) {
+          tc::tmem_ld16(taddr + (a * kOps + op) * g.acc_cols + c, v);
+          tc::tmem_ld_wait(v);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) y[j] += __uint_as_float(v[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) at[(op * g.cols + j) * kStreamFeatures] = y[j];
       }
     }
   }
@@ -589,7 +639,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
   if (aborted && threadIdx.x == 0) raise_status(p.status, kStatusTimeout);
   if (warp == 5) {
     tc::tc_fence_after();
-    tc::tmem_dealloc(tmem, kTmemCols);
+    tc::tmem_dealloc(tmem, kStreamTmem);
   }
   // Each CTA of the cluster finishes every splits-th row, adding in rank order:
   // a warp per row, four neighbouring features per lane. A warp that has read
@@ -647,7 +697,6 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
 
 template <typename T, Kind kKind, int kAct>
 int launch(const GemmParams& g, int ctas, cudaStream_t stream) {
-  const int regs = kKind == kVocab ? kLaunchRegs : 0;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(ctas));
   cfg.blockDim = dim3(kThreads);
@@ -658,11 +707,11 @@ int launch(const GemmParams& g, int ctas, cudaStream_t stream) {
   cfg.numAttrs = launch_attributes(attrs, g.pair ? 2 : 1);
   if (g.pair) {
     constexpr auto kernel = gemm_kernel<T, kKind, kAct, true>;
-    if (const cudaError_t e = allow_smem<kernel>(kSmemBudget, regs)) return static_cast<int>(e);
+    if (const cudaError_t e = allow_smem<kernel>(kSmemBudget, kLaunchRegs)) return static_cast<int>(e);
     return launch_status(cudaLaunchKernelEx(&cfg, kernel, g));
   }
   constexpr auto kernel = gemm_kernel<T, kKind, kAct, false>;
-  if (const cudaError_t e = allow_smem<kernel>(kSmemBudget, regs)) return static_cast<int>(e);
+  if (const cudaError_t e = allow_smem<kernel>(kSmemBudget, kLaunchRegs)) return static_cast<int>(e);
   return launch_status(cudaLaunchKernelEx(&cfg, kernel, g));
 }
 
@@ -771,13 +820,20 @@ StreamPlan stream_plan(const Problem& p, int ctas) {
   return plan;
 }
 
-// Whether the vocabulary head streams too: few rows, and so few tiles that a
-// cluster shares each. A CTA's sums then cover at most kVocabBlocks blocks of
-// input features (half as many again where that is the last split), as they do
-// in gemm_kernel.
-bool head_streams(const Problem& p, int ctas) {
-  return p.rows <= kStreamRows && ceil_div(ceil_div(p.inner, kBlockK), stream_plan(p, ctas).splits) <=
-                                      kVocabBlocks + kVocabBlocks / 2;
+// Accumulators of one product that a CTA's TMEM holds, a power of two columns apart.
+int stream_acc_cols(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+int stream_accs(Kind kind, int rows) {
+  return kStreamTmem / stream_acc_cols(rows) / (kind == kGated ? 2 : 1);
+}
+
+// Whether few rows stream. Their CTA's share of the input features has to fit
+// its accumulators at kSumBlocks blocks each; the vocabulary head, whose tiles
+// are many, streams where a share is at most half as many again as one holds.
+bool streams(Kind kind, const Problem& p, int ctas) {
+  if (p.rows > kStreamRows) return false;
+  const int share = ceil_div(ceil_div(p.inner, kBlockK), stream_plan(p, ctas).splits);
+  return kind == kVocab ? share <= kSumBlocks + kSumBlocks / 2
+                        : share <= kSumBlocks * stream_accs(kind, p.rows);
 }
 
 int run_stream(Kind kind, const Problem& p, int32_t dtype, int ctas, cudaStream_t stream) {
@@ -794,11 +850,14 @@ int run_stream(Kind kind, const Problem& p, int32_t dtype, int ctas, cudaStream_
   g.splits = plan.splits;
   const int kblocks = ceil_div(p.inner, kBlockK);
   const int per_cta = ceil_div(kblocks, g.splits);
+  const int accs = ceil_div(per_cta, kSumBlocks);
+  g.acc_blocks = ceil_div(per_cta, accs);
+  g.acc_cols = stream_acc_cols(p.rows);
   g.stages = plan.budget / g.stage_bytes;
   // The whole class even where less is used. CTAs of a cluster wait for one
   // another, and TMEM is handed out as it comes: were more CTAs on an SM than its
   // TMEM has room for, two clusters could each hold what the other waits for.
-  // With 110 KB two of these CTAs fit (256 of 512 columns), and none beside a
+  // With 110 KB two of these CTAs fit (256 columns each), and none beside a
   // cluster that takes all of TMEM, which asks for more than the other half.
   g.smem_bytes = plan.budget + 1024;
   if (g.stages > kStreamStages) g.stages = kStreamStages;
@@ -823,12 +882,12 @@ int run_stream(Kind kind, const Problem& p, int32_t dtype, int ctas, cudaStream_
 }  // namespace
 
 int tc_vocab_parts(const Problem& p, int ctas) {
-  if (head_streams(p, ctas)) return ceil_div(p.outer, kStreamFeatures);
+  if (streams(kVocab, p, ctas)) return ceil_div(p.outer, kStreamFeatures);
   return 2 * ceil_div(p.outer, choose_tiling(kVocab, p, ctas).set_n);
 }
 
 int run_tc(Kind kind, const Problem& p, int32_t dtype, int ctas, cudaStream_t stream) {
-  if (kind == kVocab ? head_streams(p, ctas) : p.rows <= kStreamRows)
+  if (streams(kind, p, ctas))
     return run_stream(kind, p, dtype, ctas, stream);
   GemmParams g{};
   g.p = p;
