@@ -104,6 +104,7 @@ SIGNATURES = {
     "rlt_gated_linear": (_i32, [_p] * 4 + [_sz, _p] + [_i32] * 5 + [_i64] * 4 + [_p]),
     "rlt_vocab_head_workspace_bytes": (_sz, [_p, _p] + [_i32] * 4 + [_i64] * 3),
     "rlt_vocab_head": (_i32, [_p] * 6 + [_sz, _p] + [_i32] * 4 + [_i64] * 3 + [_p]),
+    "rlt_status_create": (_i32, [ctypes.POINTER(_p)]),
     "rlt_copy_segments": (_i32, [_p, _i32, _i64, _p, _p]),
     "rlt_enable_peer_access": (_i32, [_i32]),
     "rlt_gather": (_i32, [_p, _p, _p, _i32, _i32, _i32, _i32, _i64, _i64, _p]),
@@ -158,16 +159,30 @@ def stream_of(device: torch.device) -> int:
 _status: dict[int, torch.Tensor] = {}
 
 
+class _Word:
+    """One int32 of device memory, for ``torch.as_tensor``."""
+
+    def __init__(self, address: int):
+        self.__cuda_array_interface__ = {
+            "shape": (1,), "typestr": "<i4", "data": (address, False), "version": 3}
+
+
 def status_word(device: torch.device) -> torch.Tensor:
-    """Per-device int32 word the kernels OR metadata-error bits into."""
+    """Per-device int32 word the kernels OR metadata-error bits into. It may be
+    first requested while a stream is captured: it belongs to no graph."""
     index = device.index if device.index is not None else torch.cuda.current_device()
     word = _status.get(index)
     if word is None:
+        lib = load()
         # a normal tensor even when first requested under torch.inference_mode
         # (the reference's graph runner runs there), so it can be cleared later
-        with torch.inference_mode(False):
-            word = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", index))
-        _status[index] = word
+        with _lock, torch.cuda.device(index), torch.inference_mode(False):
+            word = _status.get(index)
+            if word is None:
+                address = _p()
+                check(lib.rlt_status_create(ctypes.byref(address)), "status word")
+                word = torch.as_tensor(_Word(address.value), device=torch.device("cuda", index))
+                _status[index] = word
     return word
 
 
