@@ -342,16 +342,18 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
       // exchange (600 rows against 15776 entries: 201 us, through shared memory 284)
       const int row = m0 + (warp & 3) * 32 + lane, at = n0 + half * 64;
       const int cols = min(64, p.outer - at);
-      bool odd = false;
+      uint64_t odd = 0;
 #pragma unroll
-      for (int j = 0; j < 64; ++j) odd = odd || (j < cols && v[j] != v[j]);
-      if (odd && row < p.rows) {
-        for (int i = 0; i < cols; ++i) {
-          const float y = plain_dot(p, static_cast<const float*>(p.w), row, at + i);
+      for (int j = 0; j < 64; ++j)
+        if (j < cols && v[j] != v[j]) odd |= 1ull << j;
+      if (row >= p.rows) odd = 0;
+      while (odd != 0) {
+        const int i = __ffsll(static_cast<long long>(odd)) - 1;
+        odd &= odd - 1;
+        const float y = plain_dot(p, static_cast<const float*>(p.w), row, at + i);
 #pragma unroll
-          for (int j = 0; j < 64; ++j)
-            if (j == i && v[j] != v[j]) v[j] = y;
-        }
+        for (int j = 0; j < 64; ++j)
+          if (j == i) v[j] = y;
       }
       __syncwarp();
       const int64_t want = p.tokens != nullptr && row < p.rows ? p.tokens[row] : -1;
@@ -417,11 +419,17 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
             const float any = y[op][0] + y[op][1] + y[op][2] + y[op][3];
             if (any != any) {
               const float* w = static_cast<const float*>(op == 0 ? p.w : p.w_up);
+#pragma unroll 1
               for (int i = 0; i < 4 && n + i < p.outer; ++i) {
-                const float plain = plain_dot(p, w, m0 + r, n + i);
+                float mine = y[op][0];
+#pragma unroll
+                for (int e = 1; e < 4; ++e)
+                  if (e == i) mine = y[op][e];
+                if (mine == mine) continue;
+                mine = plain_dot(p, w, m0 + r, n + i);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                  if (e == i && y[op][e] != y[op][e]) y[op][e] = plain;
+                  if (e == i) y[op][e] = mine;
               }
             }
           }
