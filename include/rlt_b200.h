@@ -428,8 +428,9 @@ size_t rlt_linear_workspace_bytes(const void* x, const void* weight, int32_t dty
  * tensor as residual and overlaps nothing else. in_features >= 1; rows or
  * out_features of 0 launch nothing. act: RLT_ACT_*. A row's result depends on
  * that row, the weights, and the launch shape only, and repeats bit for bit.
- * All types run on the tensor cores, fp32 as three bf16 parts per number (six
- * products of parts, to about the error of fp32 multiply-adds).
+ * All types run on the tensor cores, fp32 as three bf16 parts per number: the six
+ * products of parts that are formed leave out at most 2^-24 of a product; bits of
+ * a number below 2^-133 do not count.
  * Replaces the projections of vllm_rlt/models/ouro.py:96-123 with what follows
  * them, and the exit gate's product, bias and sigmoid (:209-217). */
 int rlt_linear(const void* x, const void* weight, const void* bias, const void* residual,

@@ -42,3 +42,51 @@ def test_one_infinite_weight_costs_its_own_entry_alone(rows):
     assert tokens[up].eq(700).all() and logprobs[up].isnan().all()
     rest = ~up & before.ne(700)
     assert rest.any() and torch.equal(tokens[rest], before[rest]) and logprobs[rest].isfinite().all()
+
+
+# ------------------------------------------------------- fp32 as three bf16 parts
+
+
+def test_single_precision_products():
+    """Products of two numbers. The parts of a number leave out at most 2^-24
+    (1 + 2^-10) of a product; the sum of the large and the small ones is rounded
+    once (2^-24), and the five small products, 2^-7 of it together, truncate when
+    they meet (a step of each other at most, 5 x 2^-23 x 2^-7)."""
+    g = generator(82)
+    bits = torch.cat([torch.tensor([0x3f80ffff, 0x3f808000, 0x3f818000, 0x3fffffff, 0x3f800001]),
+                      torch.randint(0x3f800000, 0x40000000, (251,), generator=torch.Generator().manual_seed(82))])
+    x = bits.int().view(torch.float32).cuda()[:, None]
+    w = torch.cat([x, normal(g, 256, 1), -x])
+    got, want = rb.linear(x, w).double(), x.double() @ w.double().t()
+    bound = (2 + 2.0 ** -9 + 5 * 2.0 ** -6) * 2.0 ** -24
+    assert (((got - want) / want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("rows", [40, 300])
+def test_single_precision_sums_are_not_biased(rows):
+    """Sums of 64 products in [1, 4): the large ones add up exactly (16 bits above
+    2^-14, less than 2^8 together), so an output's error is that of the parts left
+    out and of one rounding, each within 2^-24 and of both signs. Over the outputs
+    of 40 x 64 or more independent numbers its mean stays below 5 x 2^-23 /
+    sqrt(2560), which is below 2^-26; parts left out with one sign leave 4e-8."""
+    g = generator(83)
+    x, w = (torch.rand(n, 64, device="cuda", generator=g) + 1 for n in (rows, 400))
+    got, want = rb.linear(x, w).double(), x.double() @ w.double().t()
+    assert abs(((got - want) / want).mean().item()) < 2.0 ** -26
+
+
+def test_single_precision_near_the_largest_number():
+    """Numbers that round up to infinity as bf16, and products whose large parts
+    overflow although the product does not, come out as fp32 multiply-adds give
+    them; the head sees the same."""
+    most = torch.finfo(torch.float32).max
+    for a, b in ((most, 1.0), (most, 0.5), (-3.4e38, 0.9999), (1.8446e19, 1.8446e19),
+                 (1.8446e19, -1.8446e19), (3.3961e38, 1.0), (2.0 ** 127 * 1.999, 1.0)):
+        for rows in (3, 200):
+            x = torch.full((rows, 1), a, device="cuda")
+            w = torch.full((70, 1), b, device="cuda")
+            want = x.double() @ w.double().t()
+            got = rb.linear(x, w).double()
+            assert torch.equal(got.isinf(), want.abs() > most) and not got.isnan().any()
+            fine = got.isfinite()
+            assert ((got - want)[fine].abs() <= 2.0 ** -22 * want[fine].abs()).all()

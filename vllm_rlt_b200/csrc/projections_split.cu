@@ -1,12 +1,18 @@
 // Projections of fp32 tensors on the tensor cores.
 //
-// An fp32 number is the sum of three bf16 numbers: its upper 8 significand bits
-// h, the next 8 m and the last 8 l, each split off by truncation, which is
-// exact. A product of two fp32 numbers is then the nine products of their
-// parts, each exact in fp32; the six of them down to 2^-16 of the largest are
-// formed (h h; h m, m h, m m, h l, l h) and what is left out is below 2^-23 of
-// the product, a rounding of fp32 arithmetic. bf16 products run 32 times as
-// fast as fp32 multiply-adds here, so six of them still are five times faster.
+// An fp32 number is the sum of three bf16 numbers: itself rounded to nearest, h,
+// what that leaves rounded to nearest, m, and the rest, l, which has 8 bits or
+// fewer. With the number in [1, 2) times a power of two, |m| <= 2^-8 and |l| <=
+// 2^-17 of that power. A product of two numbers is then the nine products of
+// their parts, each exact in fp32; the six largest are formed (h h; h m, m h, m m,
+// h l, l h), and what is left out (m l, l m, l l) is at most 2^-24 (1 + 2^-10) of
+// the product, of either sign. (Split by truncation it reaches 2^-21, always of
+// the product's sign: sums of positive numbers came out 4e-8 too small.) bf16
+// products run 32 times as fast as fp32 multiply-adds here, so six of them still
+// are five times faster.
+//
+// Bits of a number below 2^-133, bf16's smallest, are not counted: a number under
+// 2^-110 has fewer than its 24.
 //
 // The tensor core truncates as it accumulates, an error of one sign that grows
 // with the number of steps. h h and the five small products therefore have an
@@ -14,9 +20,10 @@
 // input features go into them, and those sums are added in registers, rounded
 // to nearest.
 //
-// Infinities: splitting one leaves NaN parts, so its row or column comes out as
-// NaN. Any NaN that comes out is recomputed by fp32 multiply-adds from the
-// operands, so infinities and NaN end up as they would there.
+// Infinities, and numbers that round up to one, leave NaN parts, so their row or
+// column comes out as NaN; a product within 2^-7 of the largest number may
+// overflow in h h. Whatever comes out as NaN or infinite is recomputed by fp32
+// multiply-adds from the operands, and ends up as it would there.
 //
 // A CTA (20 warps) takes a tile of 128 rows by 128 weight rows over its share of
 // the input features; a cluster of up to 8 CTAs shares a tile when there are few.
@@ -66,22 +73,28 @@ struct SplitParams {
 // Eight fp32 numbers as 3 x 8 bf16, packed in 16 bytes each.
 __device__ __forceinline__ void split8(const float4& a, const float4& b, uint4 (&part)[3]) {
   const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-  uint32_t h[8], m[8], l[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    h[e] = __float_as_uint(x[e]) & 0xffff0000u;
-    const float r = x[e] - __uint_as_float(h[e]);
-    m[e] = __float_as_uint(r) & 0xffff0000u;
-    l[e] = __float_as_uint(r - __uint_as_float(m[e]));
-  }
-  auto pack = [](const uint32_t (&v)[8]) {  // the upper halves of neighbours
-    return make_uint4(__byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632),
-                      __byte_perm(v[4], v[5], 0x7632), __byte_perm(v[6], v[7], 0x7632));
+  uint32_t h[4], m[4], l[4];
+  auto nearest = [](float lo, float hi) {
+    const __nv_bfloat162 t = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&t);
   };
-  part[0] = pack(h);
-  part[1] = pack(m);
-  part[2] = pack(l);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float r0 = x[2 * e], r1 = x[2 * e + 1];
+    h[e] = nearest(r0, r1);
+    r0 -= __uint_as_float(h[e] << 16);
+    r1 -= __uint_as_float(h[e] & 0xffff0000u);
+    m[e] = nearest(r0, r1);
+    r0 -= __uint_as_float(m[e] << 16);
+    r1 -= __uint_as_float(m[e] & 0xffff0000u);
+    l[e] = __byte_perm(__float_as_uint(r0), __float_as_uint(r1), 0x7632);  // their upper halves
+  }
+  part[0] = make_uint4(h[0], h[1], h[2], h[3]);
+  part[1] = make_uint4(m[0], m[1], m[2], m[3]);
+  part[2] = make_uint4(l[0], l[1], l[2], l[3]);
 }
+
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 
 // 64-byte-swizzled K-major tile: rows of 32 bf16, atoms of 8 rows.
 __device__ __forceinline__ uint64_t smem_desc_sw64(uint32_t addr) {
@@ -345,7 +358,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
       uint64_t odd = 0;
 #pragma unroll
       for (int j = 0; j < 64; ++j)
-        if (j < cols && v[j] != v[j]) odd |= 1ull << j;
+        if (j < cols && !finite(v[j])) odd |= 1ull << j;
       if (row >= p.rows) odd = 0;
       while (odd != 0) {
         const int i = __ffsll(static_cast<long long>(odd)) - 1;
@@ -417,7 +430,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
             y[op][2] = t[0].z;
             y[op][3] = t[0].w;
             const float any = y[op][0] + y[op][1] + y[op][2] + y[op][3];
-            if (any != any) {
+            if (!finite(any)) {
               const float* w = static_cast<const float*>(op == 0 ? p.w : p.w_up);
 #pragma unroll 1
               for (int i = 0; i < 4 && n + i < p.outer; ++i) {
@@ -425,7 +438,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
 #pragma unroll
                 for (int e = 1; e < 4; ++e)
                   if (e == i) mine = y[op][e];
-                if (mine == mine) continue;
+                if (finite(mine)) continue;
                 mine = plain_dot(p, w, m0 + r, n + i);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
