@@ -90,3 +90,31 @@ def test_single_precision_near_the_largest_number():
             assert torch.equal(got.isinf(), want.abs() > most) and not got.isnan().any()
             fine = got.isfinite()
             assert ((got - want)[fine].abs() <= 2.0 ** -22 * want[fine].abs()).all()
+
+
+# ----------------------------------------------------------------- activations
+
+
+@pytest.mark.parametrize("op", ["linear", "gated"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_gelu_of_negative_numbers(op, dtype):
+    """Relative to the result: x / sqrt 2 is rounded twice (2^-24 and 2^-25 of it),
+    which moves erfc by up to 2 u^2 = x^2 times as much, at most 36 x 1.5 x 2^-24 on
+    [-6, 0]; erfc itself is good to 4 steps of 2^-23, the products and the output
+    to half a step each. fp16 adds half of its smallest subnormal, 2^-25."""
+    x = torch.linspace(-6, 0, 16384, device="cuda").to(dtype).reshape(256, 64)
+    for rows in (40, 256):
+        z = x[:rows]
+        w = torch.eye(64, device="cuda", dtype=dtype)
+        if op == "linear":
+            got = rb.linear(z, w, activation="gelu")
+        else:  # up rows that give each row's last number: 1
+            z = torch.cat([z, torch.ones_like(z[:, :8])], 1)
+            w = torch.cat([torch.eye(72, device="cuda", dtype=dtype)[:64],
+                           torch.eye(72, device="cuda", dtype=dtype)[64:65].expand(64, 72)])
+            got = rb.gated_linear(z, w, activation="gelu")
+        z = z[:, :64].double()
+        want = 0.5 * z * torch.special.erfc(-z * 0.5 ** 0.5)
+        bound = (54 + 8 + 3) * 2.0 ** -24 + torch.finfo(dtype).eps / 2
+        small = 2.0 ** -25 if dtype == torch.float16 else 0.0
+        assert ((got.double() - want).abs() <= bound * want.abs() * (1 + bound) + small).all()

@@ -50,9 +50,11 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // Activations in fp32. For fp32 tensors through expf and a division; for
 // 16-bit ones through the hardware exponential and reciprocal, whose relative
-// error of about 2^-22 is far below the output's rounding (2^-9 for bf16,
-// 2^-12 for fp16). NaN stays NaN in each; exp overflowing to infinity gives
-// the limit (0), as the formulas do.
+// error of about 2^-22 is far below the output's rounding (2^-8 for bf16,
+// 2^-11 for fp16); a sigmoid below 2^-126 counts as 0. Gelu takes the
+// complementary error function, since 1 + erf cancels for negative x (at -5 it
+// has 4 bits left). NaN stays NaN in each; exp overflowing to infinity gives the
+// limit (0), as the formulas do.
 template <bool kPrecise>
 __device__ __forceinline__ float sigmoid_times(float x, float z) {  // x / (1 + exp(-z))
   if constexpr (kPrecise) return __fdiv_rn(x, 1.f + expf(-z));
@@ -64,7 +66,7 @@ __device__ __forceinline__ float sigmoid_times(float x, float z) {  // x / (1 + 
 template <bool kPrecise, int kAct>
 __device__ __forceinline__ float activate(float x) {
   if constexpr (kAct == RLT_ACT_SILU) return sigmoid_times<kPrecise>(x, x);
-  if constexpr (kAct == RLT_ACT_GELU) return 0.5f * x * (kPrecise ? erfcf(-x * 0.70710678f) : 1.f + erff(x * 0.70710678f));
+  if constexpr (kAct == RLT_ACT_GELU) return 0.5f * x * erfcf(-x * 0.70710678f);
   if constexpr (kAct == RLT_ACT_GELU_TANH)  // (1 + tanh u) / 2 = 1 / (1 + exp(-2u))
     return sigmoid_times<kPrecise>(x, 1.5957691216f * (x + 0.044715f * x * x * x));
   if constexpr (kAct == RLT_ACT_RELU) return x < 0.f ? 0.f : x;
