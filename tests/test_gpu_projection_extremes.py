@@ -118,3 +118,52 @@ def test_gelu_of_negative_numbers(op, dtype):
         bound = (54 + 8 + 3) * 2.0 ** -24 + torch.finfo(dtype).eps / 2
         small = 2.0 ** -25 if dtype == torch.float16 else 0.0
         assert ((got.double() - want).abs() <= bound * want.abs() * (1 + bound) + small).all()
+
+
+# ------------------------------------------------------------- vocabulary head
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [4, 70, 300])
+def test_logits_near_the_largest_number(rows, dtype):
+    """Logits of 3e38 and 1e38 beside zeros, and a row of -3e38: finite, far apart,
+    and times log2 e not a number. The likeliest entry has all of the probability
+    (shared where it is reached twice)."""
+    h = torch.zeros(rows, 64, device="cuda", dtype=dtype)
+    w = torch.zeros(900, 64, device="cuda", dtype=dtype)
+    h[:, 0] = 1e38
+    h[1, 0] = -1e38
+    w[:, 0], w[77, 0], w[500, 0], w[333, 0] = 1, 3, 3, 0
+    logits = h.double() @ w.double().t()
+    want = torch.log_softmax(logits, -1)
+    tokens, logprobs = rb.greedy_tokens(h, w)
+    assert torch.equal(tokens, logits.argmax(-1))
+    best = want.gather(1, tokens[:, None])[:, 0]
+    assert ((logprobs.double() - best).abs() <= 2.0 ** -20).all()  # of an exponential's error
+    scored = rb.token_logprobs(h, w, torch.full_like(tokens, 500)).double()
+    assert (scored[0] - best[0]).abs() <= 2.0 ** -20
+    assert (scored[1] / want[1, 500] - 1).abs() <= 2.0 ** -20
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("size", [1e4, 1e8, 1e9, 1e10, 1e20, 1e30])
+def test_large_logits(size, dtype):
+    """Entries at size, at the next smaller number of the type and at half of it:
+    from 2^28 on, where log2 e times a logit is only known to 16, the head takes
+    differences of logits first."""
+    h = torch.zeros(70, 64, device="cuda", dtype=dtype)
+    w = torch.zeros(900, 64, device="cuda", dtype=dtype)
+    h[:, 0] = 1
+    w[:, 0] = size / 2
+    w[200:, 0] = size
+    w[300, 0] = torch.nextafter(w[300, 0].cpu(), torch.zeros((), dtype=dtype)).item()
+    logits = h.double() @ w.double().t()
+    want = torch.log_softmax(logits, -1)
+    tokens, logprobs = rb.greedy_tokens(h, w)
+    assert tokens.eq(200).all()
+    # an exponential (2^-20), the roundings of a sum of 900 and of a logarithm below 7
+    assert ((logprobs.double() - want[:, 200]).abs() <= 2.0 ** -20 + 250 * 2.0 ** -24).all()
+    for token in (0, 300, 899):
+        got = rb.token_logprobs(h, w, torch.full_like(tokens, token)).double()
+        bound = 2.0 ** -20 + 250 * 2.0 ** -24 + 2.0 ** -23 * want[:, token].abs()
+        assert ((got - want[:, token]).abs() <= bound).all()

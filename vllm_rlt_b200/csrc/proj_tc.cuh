@@ -140,6 +140,14 @@ __device__ __forceinline__ VocabPart vocab_part(const Problem& p, const float (&
         }
   }
   part.sum = (s0 + s1) * ex2(-fmaf(base, kLog2e, -b));
+  // b's rounding reaches 2^-24 of it, which as an exponent has to stay small
+  const bool far = !(fabsf(b) < 268435456.f);
+  if (__any_sync(kFullMask, far)) {
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < kN; ++j) s += j < cols ? ex2((v[j] - base) * kLog2e) : 0.f;
+    if (far) part.sum = s;
+  }
   if (p.tokens != nullptr) {
     const bool here = want >= n0 && want < n0 + cols;
     if (__any_sync(kFullMask, here)) {
