@@ -167,3 +167,18 @@ def test_large_logits(size, dtype):
         got = rb.token_logprobs(h, w, torch.full_like(tokens, token)).double()
         bound = 2.0 ** -20 + 250 * 2.0 ** -24 + 2.0 ** -23 * want[:, token].abs()
         assert ((got - want[:, token]).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,vocab", [(5, 1), (70, 1), (70, 300), (200, 5000)])
+def test_probabilities_are_at_most_one(rows, vocab, dtype):
+    """Rows that are all but certain: their log-probability rounds to 0, never above."""
+    g = generator(84)
+    w = normal(g, vocab, 64, dtype=dtype)
+    h = normal(g, rows, 64) + 60 * w[torch.randint(vocab, (rows,), device="cuda", generator=g)].float()
+    h = h.to(dtype)
+    tokens, logprobs = rb.greedy_tokens(h, w)
+    assert (logprobs <= 0).all() and (rb.token_logprobs(h, w, tokens) <= 0).all()
+    assert torch.equal(rb.token_logprobs(h, w, tokens), logprobs)
+    if vocab == 1:
+        assert logprobs.eq(0).all()

@@ -54,7 +54,8 @@ __global__ void __launch_bounds__(kJoinThreads) vocab_join_kernel(
   if (threadIdx.x != 0) return;
 #pragma unroll
   for (int w = 1; w < kJoinThreads / 32; ++w) fold(a, warps[w]);
-  const float normaliser = a.most == -INFINITY ? NAN : logf(a.sum);
+  // the largest logit's own term is 1, however its sum was rounded; NaN stays
+  const float normaliser = a.most == -INFINITY ? NAN : logf(a.sum < 1.f ? 1.f : a.sum);
   if (tokens == nullptr) {
     out_tokens[row] = a.at;
     logprobs[row] = -normaliser;
