@@ -408,6 +408,10 @@ int rlt_silu_mul(const void* gate_up, void* out, int32_t dtype, int32_t rows,
 
 /* ---- projections ---- */
 
+/* Largest rows, in_features and out_features (vocab): kernels count tiles and
+ * slices past a size in 32 bits. Larger ones are RLT_E_SHAPE. */
+#define RLT_PROJ_MAX_SIZE 2147418112 /* 2^31 - 2^16 */
+
 /* Scratch of rlt_linear and rlt_gated_linear, in bytes: copies of x and of the
  * weights in rows of whole 16-byte units, for operands that are not laid out
  * so (a pointer that is not 16-byte aligned, a stride that is not a multiple

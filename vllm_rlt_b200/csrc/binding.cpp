@@ -13,6 +13,8 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <string>
+
 #include "rlt_b200.h"
 
 namespace {
@@ -45,7 +47,9 @@ int32_t dtype_code(at::ScalarType t) {
 }
 
 int32_t int32_size(int64_t n, const char* what) {
-  TORCH_CHECK_VALUE(n <= INT32_MAX, what, ": sizes must fit 32 bits");
+  // numbers as text: one streamed into the message ended the process here
+  TORCH_CHECK_VALUE(n <= RLT_PROJ_MAX_SIZE, what, ": sizes must be at most ",
+                    std::to_string(RLT_PROJ_MAX_SIZE));
   return static_cast<int32_t>(n);
 }
 
@@ -120,7 +124,7 @@ void checked(int rc, const char* what) {
   if (rc == RLT_OK) return;
   PyObject* r = PyObject_CallFunction(g_check, "is", rc, what);
   Py_XDECREF(r);
-  TORCH_CHECK(r == nullptr, what, ": error ", rc);
+  TORCH_CHECK(r == nullptr, what, ": error ", std::to_string(rc));
   throw PyError();
 }
 

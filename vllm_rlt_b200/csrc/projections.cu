@@ -209,6 +209,8 @@ int check(int32_t dtype, int32_t rows, int32_t inner, int32_t outer, int32_t act
   if (!known(dtype)) return RLT_E_DTYPE;
   if (rows < 0 || inner < 1 || outer < 0 || act < RLT_ACT_NONE || act > RLT_ACT_SIGMOID)
     return RLT_E_SHAPE;
+  if (rows > RLT_PROJ_MAX_SIZE || inner > RLT_PROJ_MAX_SIZE || outer > RLT_PROJ_MAX_SIZE)
+    return RLT_E_SHAPE;
   if (w_ns != 1 && w_ks != 1) return RLT_E_SHAPE;
   return RLT_OK;
 }

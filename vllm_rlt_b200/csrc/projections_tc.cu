@@ -908,7 +908,8 @@ int run_tc(Kind kind, const Problem& p, int32_t dtype, int ctas, cudaStream_t st
   g.ring_bytes = g.stages * g.stage_bytes + (kTileM - g.box_m) * 128;
   g.vec = aligned_to(p.out, 8) && p.o_rs % 4 == 0 && aligned_to(p.bias, 8) && aligned_to(p.residual, 8) &&
           p.r_rs % 4 == 0;
-  if (static_cast<int64_t>(g.row_tiles) * g.col_tiles > INT32_MAX) return RLT_E_SHAPE;
+  // a CTA's count of tiles steps past the last
+  if (static_cast<int64_t>(g.row_tiles) * g.col_tiles > RLT_PROJ_MAX_SIZE) return RLT_E_SHAPE;
   bool ok = encode2d(&g.map_x, dtype, p.x, p.inner, p.rows, p.x_rs, g.box_m);
   for (int half = 0; half < (kind == kGated ? 2 : 1); ++half) {
     CUtensorMap* map = half ? &g.map_up : &g.map_w;
