@@ -53,6 +53,13 @@ int32_t int32_size(int64_t n, const char* what) {
   return static_cast<int32_t>(n);
 }
 
+// A lazily negated tensor (the imaginary part of a conjugate view) holds the
+// opposite of its values, and one of lazy zeros holds none.
+void holds_values(const at::Tensor& t, const char* what) {
+  TORCH_CHECK_VALUE(!t.is_neg() && !t._is_zerotensor(), what,
+                    ": a tensor does not hold its values (resolve_neg, clone)");
+}
+
 struct Operands {
   at::Tensor x;  // rows of contiguous features
   int32_t rows, inner, outer, dtype;
@@ -69,6 +76,8 @@ Operands operands(const at::Tensor& x, const at::Tensor& w, const char* what) {
   TORCH_CHECK_VALUE(w.device() == x.device(), what, ": all tensors must live on the same device");
   TORCH_CHECK_VALUE(x.layout() == at::kStrided && w.layout() == at::kStrided, what,
                     ": tensors must be dense");
+  holds_values(x, what);
+  holds_values(w, what);
   TORCH_CHECK_VALUE(x.size(1) > 0, what, ": in_features must be positive");
   o.rows = int32_size(x.size(0), what);
   o.inner = int32_size(x.size(1), what);
@@ -92,6 +101,7 @@ void rows_like(const at::Tensor& t, int64_t outer, const Operands& o, const char
                         t.scalar_type() == o.x.scalar_type() && t.device() == o.x.device() &&
                         t.layout() == at::kStrided,
                     what, ": ", name, " must be [rows, out] of x's dtype and device");
+  holds_values(t, what);
 }
 
 void check_output(const at::Tensor* out, int64_t outer, const Operands& o, const char* what) {
@@ -149,11 +159,13 @@ at::Tensor do_linear(PyObject* const* a) {
   const at::Tensor* residual = optional(a[4], what, "residual");
   const at::Tensor* out = optional(a[5], what, "out");
   at::Tensor held_bias, held_residual, result;
-  if (bias != nullptr)
+  if (bias != nullptr) {
     TORCH_CHECK_VALUE(bias->dim() == 1 && bias->size(0) == o.outer &&
                           bias->scalar_type() == o.x.scalar_type() &&
                           bias->device() == o.x.device() && bias->layout() == at::kStrided,
                       what, ": bias must be [out] of x's dtype and device");
+    holds_values(*bias, what);
+  }
   if (residual != nullptr) rows_like(*residual, o.outer, o, "residual", what);
   check_output(out, o.outer, o, what);
   on_cuda(o, what);
