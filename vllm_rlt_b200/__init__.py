@@ -15,12 +15,14 @@ Public surface (mirrors vllm_rlt/kernels):
     residual, or with the gate's activation and product, in the same kernel;
   * ``greedy_tokens`` / ``token_logprobs`` -- language-model head reduced to
     the next token, or to given tokens' log-probabilities, without its logits;
+  * ``check_errors`` -- what kernels have reported on a device;
   * ``install`` -- put the backend into a reference KV cache manager.
 
 Importing the package does not initialise CUDA; the shared library is loaded
 on first use and its absence raises (there is no fallback path).
 """
 
+from ._lib import check_errors  # noqa: F401
 from .backend import install  # noqa: F401
 from .kernels.cache_ops import finalize, write_kv  # noqa: F401
 from .kernels.paged_attention import (  # noqa: F401

@@ -217,3 +217,14 @@ def read_status(device: torch.device, reset: bool = True) -> list[str]:
     if reset and value:
         word.zero_()
     return [text for bit, text in STATUS_BITS.items() if value & bit]
+
+
+def check_errors(device: torch.device | str | int | None = None) -> list[str]:
+    """What kernels on ``device`` (the current CUDA device by default) have reported
+    since the last look: metadata outside the pool, a token beyond the vocabulary,
+    a wait that gave up (the output of that call is void). Synchronises, and clears
+    what it returns; empty when all is well."""
+    device = torch.device("cuda" if device is None else device)
+    if device.type != "cuda":
+        raise ValueError("check_errors requires a CUDA device")
+    return read_status(device)

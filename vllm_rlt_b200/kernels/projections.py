@@ -11,8 +11,10 @@ Activations are ``[rows, features]``; weights ``[out, in]`` with either
 dimension contiguous, so a ``torch.nn.Linear`` weight and the decoder's
 transposed views (``OuroWeights``) both serve as they are. Calls launch on the
 current stream of the tensors' device, allocate only through torch and never
-synchronise, so they can be captured in a CUDA graph. There is no backward
-pass: outputs carry no gradient.
+synchronise, so they can be captured in a CUDA graph. A wait inside a kernel that
+gives up leaves its output void and is reported by
+``vllm_rlt_b200.check_errors()``. There is no backward pass: outputs carry no
+gradient.
 """
 
 from __future__ import annotations
@@ -57,8 +59,8 @@ def greedy_tokens(hidden, weight):
 def token_logprobs(hidden, weight, tokens):
     """``log_softmax(hidden @ weight.t())`` at ``tokens``, int64 ``[rows]``,
     without storing the logits; 0 where a token is negative (nothing to score).
-    A token beyond the vocabulary gives NaN and is reported by the backend's
-    ``check_errors()``. Returns fp32 ``[rows]``."""
+    A token beyond the vocabulary gives NaN and is reported by
+    ``vllm_rlt_b200.check_errors()``. Returns fp32 ``[rows]``."""
     if tokens is None:
         raise ValueError("token logprobs: tokens must be int64 [rows]")
     return _lib.native().vocab_head(hidden, weight, tokens)
