@@ -33,11 +33,13 @@
 // stream_kernel: few activation rows. The weights are what has to be read, so
 // here they are the 128-row operand and the activations the narrow one (16 to
 // 64 columns): a CTA streams 128 output features over its share of the input
-// features in TMEM accumulators of at most 512 of them, a cluster of up to 8 CTAs
+// features in TMEM accumulators of some hundred each, a cluster of up to 8 CTAs
 // shares a feature tile, and their partial sums meet in distributed shared memory:
 // each CTA reads the others' for the rows that it finishes (stored there by the
 // others with st.async instead, 64 rows took 9.4 us where reading takes 7.9). While
 // the stream's previous kernel still runs, the first weights are brought into L2.
+#include <type_traits>
+
 #include "proj_tc.cuh"
 
 namespace rlt {
@@ -55,9 +57,9 @@ constexpr int kLaunchRegs = 168, kSumRegs = 232, kOtherRegs = 40;  // per thread
 static_assert(256 * kSumRegs + 128 * kOtherRegs <= kThreads * kLaunchRegs,
               "the increase draws on what the launch allocated");
 constexpr int kStagingBytes = kEpilogueWarps * 4096;  // 32 rows x 32 fp32 columns per warp
-// 64-feature blocks accumulated in TMEM at a time: by the head and few rows, and
-// by the other tiles. With 8 the latter's next tile waits for the two accumulators
-// while outputs are stored: 4096 x 5632 -> 2048 takes 78.9 us, the gated product
+// 64-feature blocks accumulated in TMEM at a time, by the head and by the others.
+// With 8 these would wait for the two accumulators while a tile's outputs are
+// stored: 4096 x 5632 -> 2048 takes 78.9 us, the gated product
 // 4096 x 2048 -> 2 x 5632 136; with 12, 75.8 and 127; with 16, 73.9 and 124.
 constexpr int kSumBlocks = 8, kTileSumBlocks = 12;
 
@@ -462,11 +464,14 @@ struct StreamParams {
   int splits;  // CTAs per feature tile
   int smem_bytes;
   int vec;     // four neighbouring outputs (biases, residuals) are 8 aligned bytes
+  int several;     // whether a CTA's share takes more than one accumulator
   int acc_blocks;  // blocks per accumulator
-  int acc_cols;    // TMEM columns between accumulators
+  int acc_cols;    // TMEM columns between a product's accumulators
 };
 
-template <typename T, Kind kKind, int kAct>
+// kSums: a CTA's share takes more than one accumulator. (As a test within one
+// kernel it cost 64 rows with a single one 6 %.)
+template <typename T, Kind kKind, int kAct, bool kSums>
 __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_constant__ StreamParams g) {
   constexpr int kOps = kKind == kGated ? 2 : 1;
   constexpr int kBytesW = kStreamFeatures * kBlockK * 2;
@@ -555,16 +560,16 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
     const uint32_t x_hi = static_cast<uint32_t>(x_desc >> 32);
     Ring at;
     uint32_t d = tmem, more = 0;
-    int left = g.acc_blocks;  // of the present accumulator
+    int next_acc = kb0 + g.acc_blocks;
     for (int kb = kb0; kb < kb1; ++kb, at.next(g.stages)) {
-      if (left-- == 0) {
-        left = g.acc_blocks - 1;
-        d += kOps * g.acc_cols;
-        more = 0;
-      }
       if (!__all_sync(kFullMask, tc::mbar_poll(&full[at.slot], at.parity, kWaitLimit))) {
         ok = false;
         break;
+      }
+      if (kSums && kb == next_acc) {
+        next_acc += g.acc_blocks;
+        d += g.acc_cols;
+        more = 0;
       }
       tc::tc_fence_after();
       if (tc::elect_one()) {
@@ -574,7 +579,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
         for (int ks = 0; ks < kBlockK / 16; ++ks)
 #pragma unroll
           for (int op = 0; op < kOps; ++op)
-            tc::mma_f16_ss(d + op * g.acc_cols,
+            tc::mma_f16_ss(d + op * (kStreamTmem / kOps),
                            tc::desc64(w_lo + op * (kBytesW >> 4) + ks * kstep_w, w_hi),
                            tc::desc64(x_lo + ks * 2, x_hi), idesc, ks > 0 ? 1 : more);
         tc::mma_commit(&empty[at.slot]);
@@ -602,27 +607,27 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
     ok = __all_sync(kFullMask, tc::mbar_wait(&acc_full, 0, whole_sum_limit(kb1 - kb0)));
     tc::tc_fence_after();
     const uint32_t taddr = tmem + (static_cast<uint32_t>(warp) << 21);
-    for (int c = 0; ok && c < p.rows; c += 16) {
-      float* at = sums + c * kStreamFeatures + threadIdx.x;
+    auto gather = [&](uint32_t from, auto add) {
+      for (int c = 0; ok && c < p.rows; c += 16) {
+        float* at = sums + c * kStreamFeatures + threadIdx.x;
 #pragma unroll
-      for (int op = 0; op < kOps; ++op) {
-        uint32_t v[16];
-        float y[16];
-        __syncwarp();
-        tc::tmem_ld16(taddr + op * g.acc_cols + c, v);
-        tc::tmem_ld_wait(v);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) y[j] = __uint_as_float(v[j]);
-        for (int a = 1; a * g.acc_blocks < kb1 - kb0; ++a) {
-          tc::tmem_ld16(taddr + (a * kOps + op) * g.acc_cols + c, v);
+        for (int op = 0; op < kOps; ++op) {
+          uint32_t v[16];
+          __syncwarp();
+          tc::tmem_ld16(from + op * (kStreamTmem / kOps) + c, v);
           tc::tmem_ld_wait(v);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) y[j] += __uint_as_float(v[j]);
+          for (int j = 0; j < 16; ++j) {
+            float* to = at + (op * g.cols + j) * kStreamFeatures;
+            *to = add() ? *to + __uint_as_float(v[j]) : __uint_as_float(v[j]);
+          }
         }
-#pragma unroll
-        for (int j = 0; j < 16; ++j) at[(op * g.cols + j) * kStreamFeatures] = y[j];
       }
-    }
+    };
+    gather(taddr, std::false_type());
+    if constexpr (kSums)
+      for (int a = 1; a * g.acc_blocks < kb1 - kb0; ++a)
+        gather(taddr + a * g.acc_cols, std::true_type());
   }
   if (!ok) {  // a wait ran out: let copies in flight land before the memory goes
     aborted = 1;
@@ -759,8 +764,6 @@ Tiling choose_tiling(Kind kind, const Problem& p, int ctas) {
 
 template <typename T, Kind kKind, int kAct>
 int launch(const StreamParams& g, int tiles, cudaStream_t stream) {
-  constexpr auto kernel = stream_kernel<T, kKind, kAct>;
-  if (const cudaError_t e = allow_smem<kernel>(kSmemBudget)) return static_cast<int>(e);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(tiles * g.splits));
   cfg.blockDim = dim3(kStreamThreads);
@@ -769,6 +772,13 @@ int launch(const StreamParams& g, int tiles, cudaStream_t stream) {
   cudaLaunchAttribute attrs[2];
   cfg.attrs = attrs;
   cfg.numAttrs = launch_attributes(attrs, g.splits);
+  if (g.several) {
+    constexpr auto kernel = stream_kernel<T, kKind, kAct, true>;
+    if (const cudaError_t e = allow_smem<kernel>(kSmemBudget)) return static_cast<int>(e);
+    return launch_status(cudaLaunchKernelEx(&cfg, kernel, g));
+  }
+  constexpr auto kernel = stream_kernel<T, kKind, kAct, false>;
+  if (const cudaError_t e = allow_smem<kernel>(kSmemBudget)) return static_cast<int>(e);
   return launch_status(cudaLaunchKernelEx(&cfg, kernel, g));
 }
 
@@ -798,7 +808,7 @@ StreamPlan stream_plan(const Problem& p, int ctas) {
   double least = 1e300;
   for (int s = 1; s <= kMaxSplits && s <= kblocks; ++s) {
     for (int big = 0; big < 2; ++big) {
-      constexpr auto kernel = stream_kernel<__half, kLinear, RLT_ACT_NONE>;
+      constexpr auto kernel = stream_kernel<__half, kLinear, RLT_ACT_NONE, false>;
       int waves;
       if (big) {
         if (s > 6) continue;
@@ -820,20 +830,19 @@ StreamPlan stream_plan(const Problem& p, int ctas) {
   return plan;
 }
 
-// Accumulators of one product that a CTA's TMEM holds, a power of two columns apart.
-int stream_acc_cols(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
-int stream_accs(Kind kind, int rows) {
-  return kStreamTmem / stream_acc_cols(rows) / (kind == kGated ? 2 : 1);
-}
+// Blocks that an accumulator takes, and the columns between accumulators.
+int stream_acc_blocks(Kind kind) { return kind == kVocab ? kSumBlocks : kTileSumBlocks; }
+int stream_acc_cols(const Problem& p) { return p.rows <= 16 ? 16 : p.rows <= 32 ? 32 : 64; }
 
 // Whether few rows stream. Their CTA's share of the input features has to fit
-// its accumulators at kSumBlocks blocks each; the vocabulary head, whose tiles
-// are many, streams where a share is at most half as many again as one holds.
+// its accumulators; the vocabulary head, whose tiles are many, streams where a
+// share is at most half as many again as one holds.
 bool streams(Kind kind, const Problem& p, int ctas) {
   if (p.rows > kStreamRows) return false;
   const int share = ceil_div(ceil_div(p.inner, kBlockK), stream_plan(p, ctas).splits);
-  return kind == kVocab ? share <= kSumBlocks + kSumBlocks / 2
-                        : share <= kSumBlocks * stream_accs(kind, p.rows);
+  if (kind == kVocab) return share <= kSumBlocks + kSumBlocks / 2;
+  const int accs = kStreamTmem / (kind == kGated ? 2 : 1) / stream_acc_cols(p);
+  return share <= accs * stream_acc_blocks(kind);
 }
 
 int run_stream(Kind kind, const Problem& p, int32_t dtype, int ctas, cudaStream_t stream) {
@@ -850,9 +859,10 @@ int run_stream(Kind kind, const Problem& p, int32_t dtype, int ctas, cudaStream_
   g.splits = plan.splits;
   const int kblocks = ceil_div(p.inner, kBlockK);
   const int per_cta = ceil_div(kblocks, g.splits);
-  const int accs = ceil_div(per_cta, kSumBlocks);
+  const int accs = ceil_div(per_cta, stream_acc_blocks(kind));
+  g.several = accs > 1;
   g.acc_blocks = ceil_div(per_cta, accs);
-  g.acc_cols = stream_acc_cols(p.rows);
+  g.acc_cols = stream_acc_cols(p);
   g.stages = plan.budget / g.stage_bytes;
   // The whole class even where less is used. CTAs of a cluster wait for one
   // another, and TMEM is handed out as it comes: were more CTAs on an SM than its
