@@ -68,10 +68,11 @@ extern "C" {
 #define RLT_STATUS_LAYOUT 64  /* a tensor-core kernel found its shared memory misaligned */
 #define RLT_STATUS_BAD_TOKEN 128 /* a token to score lies outside the vocabulary */
 
-/* A zeroed status word on the current device, for the life of the process.
- * Also while the calling thread captures a stream: nothing of it becomes part
- * of the graph. Synchronises a stream of its own. */
-int rlt_status_create(int32_t** word);
+/* The current device's status word: one for the life of the process, clear when
+ * it is first asked for (which allocates it, and synchronises a stream of its
+ * own). Also while the calling thread captures a stream: nothing of it becomes
+ * part of the graph. */
+int rlt_status_word(int32_t** word);
 
 /* Library version (major*10000 + minor*100 + patch). */
 int rlt_version(void);

@@ -10,6 +10,7 @@ from pathlib import Path
 import pytest
 import torch
 
+import vllm_rlt_b200 as rb
 from vllm_rlt_b200 import _lib
 
 pytestmark = pytest.mark.gpu
@@ -63,3 +64,15 @@ def test_it_is_one_tensor_per_device():
     assert word.shape == (1,) and word.dtype == torch.int32 and word.device == device
     word.fill_(2)
     assert _lib.read_status(device) == [_lib.STATUS_BITS[2]] and word.item() == 0
+
+
+def test_every_entry_reports_into_the_same_word():
+    """Whoever asked first: the extension's calls, and a tensor made anew."""
+    h = torch.randn(2, 64, device="cuda").bfloat16()
+    w = torch.randn(100, 64, device="cuda").bfloat16()
+    bad = torch.tensor([5, 100], device="cuda")
+    rb.token_logprobs(h, w, bad)
+    _lib._status.pop(0, None)
+    assert rb.check_errors() == [_lib.STATUS_BITS[128]]
+    rb.token_logprobs(h, w, bad)
+    assert rb.check_errors() == [_lib.STATUS_BITS[128]] and rb.check_errors() == []

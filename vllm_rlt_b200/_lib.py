@@ -104,7 +104,7 @@ SIGNATURES = {
     "rlt_gated_linear": (_i32, [_p] * 4 + [_sz, _p] + [_i32] * 5 + [_i64] * 4 + [_p]),
     "rlt_vocab_head_workspace_bytes": (_sz, [_p, _p] + [_i32] * 4 + [_i64] * 3),
     "rlt_vocab_head": (_i32, [_p] * 6 + [_sz, _p] + [_i32] * 4 + [_i64] * 3 + [_p]),
-    "rlt_status_create": (_i32, [ctypes.POINTER(_p)]),
+    "rlt_status_word": (_i32, [ctypes.POINTER(_p)]),
     "rlt_copy_segments": (_i32, [_p, _i32, _i64, _p, _p]),
     "rlt_enable_peer_access": (_i32, [_i32]),
     "rlt_gather": (_i32, [_p, _p, _p, _i32, _i32, _i32, _i32, _i64, _i64, _p]),
@@ -180,7 +180,7 @@ def status_word(device: torch.device) -> torch.Tensor:
             word = _status.get(index)
             if word is None:
                 address = _p()
-                check(lib.rlt_status_create(ctypes.byref(address)), "status word")
+                check(lib.rlt_status_word(ctypes.byref(address)), "status word")
                 word = torch.as_tensor(_Word(address.value), device=torch.device("cuda", index))
                 _status[index] = word
     return word
@@ -204,8 +204,7 @@ def native():
                 spec = importlib.util.spec_from_file_location("_rlt_torch", BINDING_PATH)
                 module = importlib.util.module_from_spec(spec)
                 spec.loader.exec_module(module)
-                module.setup(
-                    lambda index: status_word(torch.device("cuda", index)).data_ptr(), check)
+                module.setup(check)
                 _native = module
     return _native
 

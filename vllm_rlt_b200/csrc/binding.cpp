@@ -19,11 +19,7 @@
 
 namespace {
 
-PyObject* g_status_ptr = nullptr;  // callable: torch.device -> address of its status word
-PyObject* g_check = nullptr;       // callable: (return code, what) -> raises
-
-constexpr int kDevices = 64;
-int64_t g_status[kDevices];
+PyObject* g_check = nullptr;  // callable: (return code, what) -> raises
 
 struct PyError {};  // a Python exception is set
 
@@ -117,25 +113,19 @@ void on_cuda(Operands& o, const char* what) {
   o.x_rs = o.x.stride(0);
 }
 
-int32_t* status_of(const at::Tensor& t) {
-  const int index = t.get_device();
-  if (index >= 0 && index < kDevices && g_status[index] != 0)
-    return reinterpret_cast<int32_t*>(g_status[index]);
-  PyObject* n = PyObject_CallFunction(g_status_ptr, "i", index);
-  if (n == nullptr) throw PyError();
-  const int64_t at = PyLong_AsLongLong(n);
-  Py_DECREF(n);
-  if (at == -1 && PyErr_Occurred()) throw PyError();
-  if (index >= 0 && index < kDevices) g_status[index] = at;
-  return reinterpret_cast<int32_t*>(at);
-}
-
 void checked(int rc, const char* what) {
   if (rc == RLT_OK) return;
   PyObject* r = PyObject_CallFunction(g_check, "is", rc, what);
   Py_XDECREF(r);
   TORCH_CHECK(r == nullptr, what, ": error ", std::to_string(rc));
   throw PyError();
+}
+
+// The current device's.
+int32_t* status_word(const char* what) {
+  int32_t* word = nullptr;
+  checked(rlt_status_word(&word), what);
+  return word;
 }
 
 at::Tensor scratch(size_t bytes, const at::Tensor& like) {
@@ -175,7 +165,7 @@ at::Tensor do_linear(PyObject* const* a) {
     held_residual = residual->stride(1) == 1 ? *residual : residual->contiguous();
   result = out != nullptr ? *out : at::empty({o.rows, o.outer}, o.x.options());
   if (o.rows == 0 || o.outer == 0) return result;
-  int32_t* status = status_of(o.x);
+  int32_t* status = status_word(what);
   const size_t need = rlt_linear_workspace_bytes(o.x.data_ptr(), w.data_ptr(), o.dtype, o.rows,
                                                  o.inner, o.outer, 0, o.x_rs, o.w_ns, o.w_ks);
   const at::Tensor work = scratch(need, o.x);
@@ -201,7 +191,7 @@ at::Tensor do_gated(PyObject* const* a) {
   c10::cuda::CUDAGuard guard(o.x.device());
   at::Tensor result = out != nullptr ? *out : at::empty({o.rows, outer}, o.x.options());
   if (o.rows == 0 || outer == 0) return result;
-  int32_t* status = status_of(o.x);
+  int32_t* status = status_word(what);
   const size_t need = rlt_linear_workspace_bytes(o.x.data_ptr(), w.data_ptr(), o.dtype, o.rows,
                                                  o.inner, outer, 1, o.x_rs, o.w_ns, o.w_ks);
   const at::Tensor work = scratch(need, o.x);
@@ -235,7 +225,7 @@ std::pair<at::Tensor, at::Tensor> do_head(PyObject* const* a) {
     chosen = at::empty({o.rows}, o.x.options().dtype(at::kLong));
   at::Tensor logprobs = at::empty({o.rows}, o.x.options().dtype(at::kFloat));
   if (o.rows == 0) return {chosen, logprobs};
-  int32_t* status = status_of(o.x);
+  int32_t* status = status_word(what);
   const size_t need = rlt_vocab_head_workspace_bytes(o.x.data_ptr(), w.data_ptr(), o.dtype, o.rows,
                                                      o.inner, o.outer, o.x_rs, o.w_ns, o.w_ks);
   const at::Tensor work = scratch(need, o.x);
@@ -295,11 +285,9 @@ PyObject* py_head(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 PyObject* py_setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (!arguments(n, 2)) return nullptr;
+  if (!arguments(n, 1)) return nullptr;
   Py_INCREF(a[0]);
-  Py_INCREF(a[1]);
-  Py_XSETREF(g_status_ptr, a[0]);
-  Py_XSETREF(g_check, a[1]);
+  Py_XSETREF(g_check, a[0]);
   Py_RETURN_NONE;
 }
 
@@ -307,7 +295,7 @@ PyObject* py_setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
   {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fn)), METH_FASTCALL, doc}
 
 PyMethodDef methods[] = {
-    RLT_METHOD("setup", py_setup, "setup(status_ptr, check)"),
+    RLT_METHOD("setup", py_setup, "setup(check)"),
     RLT_METHOD("linear", py_linear, "linear(x, weight, bias, activation, residual, out)"),
     RLT_METHOD("gated_linear", py_gated, "gated_linear(x, weight, activation, out)"),
     RLT_METHOD("vocab_head", py_head, "vocab_head(hidden, weight, tokens)"),

@@ -1,15 +1,18 @@
-// The status word: where kernels report what they could not raise.
+// The status words: where kernels report what they could not raise.
+#include <mutex>
+
 #include "common.cuh"
+
+namespace rlt {
+namespace {
 
 // Allocated and cleared outside of whatever the calling thread captures. A word
 // from a captured allocation would lie in that graph's pool, unset until the
 // first replay, and its clearing would be a node that every replay repeats.
-extern "C" int rlt_status_create(int32_t** word) {
-  if (word == nullptr) return RLT_E_SHAPE;
-  *word = nullptr;
+cudaError_t create(int32_t** word) {
   cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
   cudaError_t err = cudaThreadExchangeStreamCaptureMode(&mode);
-  if (err != cudaSuccess) return static_cast<int>(err);
+  if (err != cudaSuccess) return err;
   cudaStream_t stream = nullptr;
   void* at = nullptr;
   err = cudaStreamCreateWithFlags(&stream, cudaStreamNonBlocking);
@@ -24,5 +27,24 @@ extern "C" int rlt_status_create(int32_t** word) {
   }
   (void)cudaThreadExchangeStreamCaptureMode(&mode);
   *word = static_cast<int32_t*>(at);
+  return err;
+}
+
+}  // namespace
+}  // namespace rlt
+
+extern "C" int rlt_status_word(int32_t** word) {
+  constexpr int kDevices = 64;
+  static std::mutex lock;
+  static int32_t* words[kDevices];
+  if (word == nullptr) return RLT_E_SHAPE;
+  *word = nullptr;
+  int dev = 0;
+  if (const cudaError_t err = cudaGetDevice(&dev)) return static_cast<int>(err);
+  if (dev < 0 || dev >= kDevices) return RLT_E_DEVICE;
+  lock.lock();  // nothing below throws
+  const cudaError_t err = words[dev] != nullptr ? cudaSuccess : rlt::create(&words[dev]);
+  *word = words[dev];
+  lock.unlock();
   return static_cast<int>(err);
 }
