@@ -802,7 +802,8 @@ StreamPlan stream_plan(const Problem& p, int ctas) {
   // die's parts) or two of 110 KB. The partial sums of many rows cost more to
   // exchange in wide clusters: at 64 rows 3 x 200 KB takes 14.1 us for the gated
   // product and 6 x 110 KB 15.9, while one row takes 11.6 and 10.9; 64 rows of
-  // 2048 x 2048 take 6.9 us with 6 x 200 KB and 7.6 with 8 x 110 KB.
+  // 2048 x 2048 take 6.9 us with 6 x 200 KB and 7.6 with 8 x 110 KB. The border at
+  // 16 rows lies between those sizes.
   const bool many = p.rows > 16;
   constexpr int kBig = 200 * 1024, kSmall = 110 * 1024;
   double least = 1e300;
